@@ -101,6 +101,76 @@ class K3HipMoeSpineV1(C.Structure):
     ]
 
 
+class K3HipLinearV1(C.Structure):
+    _fields_ = [
+        ("abi_version", C.c_uint32),
+        ("struct_bytes", C.c_uint32),
+        ("matrix_kind", C.c_uint32),
+        ("activation", C.c_uint32),
+        ("x_dtype", C.c_uint32),
+        ("out_dtype", C.c_uint32),
+        ("rows", C.c_uint32),
+        ("columns", C.c_uint32),
+        ("positions", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("weights", C.c_void_p),
+        ("row_scales", C.c_void_p),
+        ("bias", C.c_void_p),
+        ("x", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("out", C.c_void_p),
+    ]
+
+
+class K3HipGatedV1(C.Structure):
+    _fields_ = [
+        ("abi_version", C.c_uint32),
+        ("struct_bytes", C.c_uint32),
+        ("matrix_kind", C.c_uint32),
+        ("activation", C.c_uint32),
+        ("x_dtype", C.c_uint32),
+        ("out_dtype", C.c_uint32),
+        ("rows", C.c_uint32),
+        ("columns", C.c_uint32),
+        ("positions", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("gate", C.c_void_p),
+        ("up", C.c_void_p),
+        ("gate_scales", C.c_void_p),
+        ("up_scales", C.c_void_p),
+        ("x", C.c_void_p),
+        ("out", C.c_void_p),
+        ("out_gate", C.c_void_p),
+        ("out_up", C.c_void_p),
+    ]
+
+
+class K3HipGatedGradV1(C.Structure):
+    _fields_ = [
+        ("abi_version", C.c_uint32),
+        ("struct_bytes", C.c_uint32),
+        ("activation", C.c_uint32),
+        ("dtype", C.c_uint32),
+        ("rows", C.c_uint32),
+        ("columns", C.c_uint32),
+        ("positions", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("gate", C.c_void_p),
+        ("up", C.c_void_p),
+        ("x", C.c_void_p),
+        ("g", C.c_void_p),
+        ("u", C.c_void_p),
+        ("grad", C.c_void_p),
+        ("d_x", C.c_void_p),
+        ("d_gate", C.c_void_p),
+        ("d_up", C.c_void_p),
+    ]
+
+
+K3_DENSE_ABI_V1 = 1
+K3_DENSE_MAX_EXTENT = 1048576
+K3_DENSE_ACT_NONE, K3_DENSE_ACT_SILU, K3_DENSE_ACT_GELU = 0, 1, 2
+
 K3_SPINE_MATRIX_BF16 = 0
 K3_SPINE_MATRIX_INT8 = 1
 K3_MOE_SPINE_ABI_V1 = 1
@@ -122,6 +192,9 @@ K3_HIP_CACHE_MAX_EXPERTS = 1472  # 92 strata x 16 (provider_cuda_moe.cpp:55-57)
 assert C.sizeof(K3HipCachePolicyV1) == 32
 
 assert C.sizeof(K3HipMoeSpineV1) == 144
+assert C.sizeof(K3HipLinearV1) == 88
+assert C.sizeof(K3HipGatedV1) == 104
+assert C.sizeof(K3HipGatedGradV1) == 104
 assert C.sizeof(K3HipKernelTimingV1) == 64
 assert C.sizeof(K3HipExpertDescriptorV1) == 32
 assert C.sizeof(K3HipGeometryV1) == 32
@@ -210,6 +283,13 @@ SIGNATURES = {
     "k3_hip_spine_bf16_decode_bits": (_i32, [_vp, _vp, _i32, _vp]),
     "k3_hip_spine_int8_launch_v1": (_i32, [_vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp]),
     "k3_hip_rms_norm": (_i32, [_vp, _vp, _vp, _i32, _i32, C.c_float, _vp]),
+    # include/k3_hip_dense_abi.h
+    "k3_hip_linear_workspace_bytes": (_u64, [C.POINTER(K3HipLinearV1)]),
+    "k3_hip_linear": (_i32, [C.POINTER(K3HipLinearV1), _vp, _u64, _vp]),
+    "k3_hip_gated_ffn_workspace_bytes": (_u64, [C.POINTER(K3HipGatedV1)]),
+    "k3_hip_gated_ffn": (_i32, [C.POINTER(K3HipGatedV1), _vp, _u64, _vp]),
+    "k3_hip_gated_ffn_grad_workspace_bytes": (_u64, [C.POINTER(K3HipGatedGradV1)]),
+    "k3_hip_gated_ffn_grad": (_i32, [C.POINTER(K3HipGatedGradV1), _vp, _u64, _vp]),
 }
 
 _LIB: C.CDLL | None = None

@@ -1,0 +1,713 @@
+// Dense layers over many positions on the BF16 matrix cores: a projection with bias,
+// activation and residual, the gated feed-forward block and its gradient
+// (include/k3_hip_dense_abi.h).  The product core is k3_gemm.h; this file lays operands
+// out, ends the sums and chooses tiles.
+//
+// fp32 activations.  x = t0 + t1 + t2, each term the BF16 nearest to what the earlier
+// ones leave (24 bits in all), written once as three planes; a product is then three
+// segments of the same sum.  Forward rows are first scaled by a power of two that brings
+// their largest value into [1, 2), so that no term of a value within 2^-100 of it falls
+// below BF16's smallest subnormal; the sum's end takes the scale back.
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <algorithm>
+
+#include "k3_dense.h"
+#include "k3_device.h"
+#include "k3_gemm.h"
+#include "k3_internal.h"
+#include "k3_launch.h"
+
+namespace k3 {
+namespace {
+
+using namespace gemm;
+
+enum { EPI_LINEAR = 0, EPI_GLU = 1, EPI_GRAD = 2 };
+
+// What happens to a sum.
+struct Epilogue {
+  const float* rs;    // int8 row scales [n]
+  const float* rs2;   // GLU: up's
+  const float* bias;  // LINEAR
+  const float* xs;    // [m] scale of an fp32 activation row
+  const void* res;    // LINEAR
+  void* out;          // [m][n]; GRAD with half: rows [0, half) of m
+  void* out1;         // GLU: kept g; GRAD: rows [half, 2 half)
+  void* out2;         // GLU: kept u
+  int n, m;           // outputs of a row and rows (GRAD with half: 2 half)
+  int half, valid;    // GRAD: rows per matrix and those that exist; half 0: one matrix
+  int act, bf16;      // output type
+  int vec;            // four neighbours of a row are one aligned access
+};
+
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  typedef float v2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2{a, b}, v2bf));
+}
+
+// Columns n .. n + 3 (those below e.n) of a row that starts at element `row`.
+__device__ __forceinline__ void store4(const Epilogue& e, void* out, uint64_t row, int n,
+                                       f32x4 v) {
+  if (e.vec && n + 4 <= e.n) {
+    if (e.bf16)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + row + n) =
+          make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+    else
+      *reinterpret_cast<f32x4*>(static_cast<float*>(out) + row + n) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n + i >= e.n) break;
+    if (e.bf16)
+      static_cast<uint16_t*>(out)[row + n + i] = (uint16_t)bf16_pair(v[i], 0.f);
+    else
+      static_cast<float*>(out)[row + n + i] = v[i];
+  }
+}
+
+__device__ __forceinline__ f32x4 load4(const Epilogue& e, const void* p, int bf16, uint64_t row,
+                                       int n) {
+  f32x4 v = {0.f, 0.f, 0.f, 0.f};
+  if (e.vec && n + 4 <= e.n) {
+    if (!bf16) return *reinterpret_cast<const f32x4*>(static_cast<const float*>(p) + row + n);
+    const uint2 b = *reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(p) + row + n);
+    return f32x4{__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u),
+                 __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u)};
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if (n + i >= e.n) break;
+    v[i] = bf16 ? __uint_as_float((uint32_t) static_cast<const uint16_t*>(p)[row + n + i] << 16)
+                : static_cast<const float*>(p)[row + n + i];
+  }
+  return v;
+}
+
+__device__ __forceinline__ float unary(int act, float z) {
+  if (act == K3_DENSE_ACT_SILU) return z / (1.0f + expf(-z));
+  if (act == K3_DENSE_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
+  return z;
+}
+
+// Sums v (GLU: of gate, u of up) of row m, columns n .. n + 3.
+template <int EPI>
+__device__ __forceinline__ void finish(const Epilogue& e, int m, int n, f32x4 v, f32x4 u) {
+  if (n >= e.n || m >= e.m) return;
+  if constexpr (EPI == EPI_GRAD) {
+    void* out = e.out;
+    int r = m;
+    if (e.half) {
+      if (m >= e.half) {
+        out = e.out1;
+        r = m - e.half;
+      }
+      if (r >= e.valid) return;
+    }
+    store4(e, out, (uint64_t)r * e.n, n, v);
+    return;
+  }
+  const uint64_t row = (uint64_t)m * e.n;
+  if (e.xs) {
+    const float s = e.xs[m];
+    v *= s;
+    if constexpr (EPI == EPI_GLU) u *= s;
+  }
+  if (e.rs) {
+    v *= load4(e, e.rs, 0, 0, n);
+    if constexpr (EPI == EPI_GLU) u *= load4(e, e.rs2, 0, 0, n);
+  }
+  if constexpr (EPI == EPI_GLU) {
+    f32x4 h;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = activate(e.act, v[i], u[i]);
+    if (e.out1) {
+      store4(e, e.out1, row, n, v);
+      store4(e, e.out2, row, n, u);
+    }
+    store4(e, e.out, row, n, h);
+  } else {
+    if (e.bias) v += load4(e, e.bias, 0, 0, n);
+    if (e.act != K3_DENSE_ACT_NONE) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] = unary(e.act, v[i]);
+    }
+    if (e.res) v += load4(e, e.res, e.bf16, row, n);
+    store4(e, e.out, row, n, v);
+  }
+}
+
+// part: [splits][m][pitch] sums of a split K, in place of the epilogue.  With GLU the
+// pitch runs over blocks of 16 gate and 16 up columns.
+template <int BN, int BM, int NWN, int NWM, int WL, int XL, int EPI>
+__global__ __launch_bounds__(64 * NWN * NWM) void k_gemm(const GemmArgs a, const Epilogue e,
+                                                         float* part, int pitch) {
+  constexpr bool kGlu = EPI == EPI_GLU;
+  typedef Core<BN, BM, NWN, NWM, WL, XL, kGlu> C;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * C::kBuffer];
+  int tn, tm;
+  tile_of(blockIdx.x, a.tiles_n, a.tiles_m, &tn, &tm);
+  f32x4 acc[C::FN][C::FM];
+  C::run(a, lds, tn, tm, blockIdx.y, acc);
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int nb = tn * BN + (wave % NWN) * C::FN * 16 + 4 * (lane >> 4);  // GLU: of pair columns
+  const int mb = tm * BM + (wave / NWN) * C::FM * 16 + (lane & 15);
+  if (part) {
+#pragma unroll
+    for (int j = 0; j < C::FM; ++j) {
+      const int m = mb + 16 * j;
+      if (m >= a.m) continue;
+      float* row = part + ((uint64_t)blockIdx.y * a.m + m) * pitch;
+#pragma unroll
+      for (int i = 0; i < C::FN; ++i)
+        if (nb + 16 * i < pitch) *reinterpret_cast<f32x4*>(row + nb + 16 * i) = acc[i][j];
+    }
+    return;
+  }
+  if constexpr (kGlu) {
+    const int n0 = (tn * BN + (wave % NWN) * C::FN * 16) / 2 + 4 * (lane >> 4);
+#pragma unroll
+    for (int j = 0; j < C::FM; ++j)
+#pragma unroll
+      for (int i = 0; i < C::FN; i += 2)
+        finish<EPI>(e, mb + 16 * j, n0 + 8 * i, acc[i][j], acc[i + 1][j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < C::FM; ++j)
+#pragma unroll
+      for (int i = 0; i < C::FN; ++i)
+        finish<EPI>(e, mb + 16 * j, nb + 16 * i, acc[i][j], f32x4{});
+  }
+}
+
+// The splits' sums in order, then the epilogue: four columns of one row per thread.
+template <int EPI>
+__global__ __launch_bounds__(256) void k_gemm_join(const Epilogue e, const float* part, int splits,
+                                                   int pitch) {
+  const int quads = (e.n + 3) / 4;
+  const uint64_t total = (uint64_t)e.m * quads;
+  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
+    const int m = (int)(t / quads), n = 4 * (int)(t % quads);
+    const uint64_t at =
+        (uint64_t)m * pitch + (EPI == EPI_GLU ? (uint32_t)(n >> 4) * 32 + (n & 15) : n);
+    f32x4 v = {0.f, 0.f, 0.f, 0.f}, u = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+      const float* p = part + (uint64_t)s * e.m * pitch + at;
+      v += *reinterpret_cast<const f32x4*>(p);
+      if constexpr (EPI == EPI_GLU) u += *reinterpret_cast<const f32x4*>(p + 16);
+    }
+    finish<EPI>(e, m, n, v, u);
+  }
+}
+
+// ------------------------------------------------------------------ operand layout
+// Nearest BF16 of a finite value (the largest finite one where that overflows), an
+// infinity or a quiet NaN of the others.
+__device__ __forceinline__ uint32_t nearest_bf16(float v) {
+  const uint32_t u = __float_as_uint(v);
+  if ((u & 0x7f800000u) == 0x7f800000u)
+    return (u >> 16) | ((u & 0x7fffffu) ? 0x40u : 0u);
+  const uint32_t r = (u + 0x7fffu + ((u >> 16) & 1u)) >> 16;
+  return (r & 0x7f80u) == 0x7f80u ? u >> 16 : r;
+}
+
+// Three BF16 terms of v; only the first of an infinity or NaN.
+__device__ __forceinline__ void terms3(float v, uint32_t (&t)[3]) {
+  t[0] = nearest_bf16(v);
+  t[1] = t[2] = 0u;
+  if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) return;
+  const float r = v - __uint_as_float(t[0] << 16);
+  t[1] = nearest_bf16(r);
+  t[2] = nearest_bf16(r - __uint_as_float(t[1] << 16));
+}
+
+// fp32 rows to three planes [3][rows][pitch / 2] (pitch in bytes, zeros past cols); with
+// xs, scaled by the power of two that brings the row's largest finite value into
+// [1, 2), whose inverse goes to xs[row].
+__global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x,
+                                                    uint8_t* __restrict__ planes,
+                                                    float* __restrict__ xs, int rows, int cols,
+                                                    uint32_t pitch) {
+  const uint64_t plane = (uint64_t)rows * pitch;
+  __shared__ float red[4];
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float* p = x + (uint64_t)row * cols;
+    float scale = 1.f;
+    if (xs) {
+      float most = 0.f;
+      for (int c = threadIdx.x; c < cols; c += 256) {
+        const float a = fabsf(p[c]);
+        if (a < INFINITY) most = fmaxf(most, a);
+      }
+#pragma unroll
+      for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+      __syncthreads();  // red of the row before
+      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+      __syncthreads();
+      most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+      // exponents -126 .. 126, so that the scale and its inverse are normal numbers
+      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
+      if (most > 0.f) scale = __uint_as_float((uint32_t)(127 - e) << 23);
+      if (threadIdx.x == 0) xs[row] = most > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+    }
+    uint32_t* d = reinterpret_cast<uint32_t*>(planes + (uint64_t)row * pitch);
+    for (int c = 2 * threadIdx.x; c < (int)(pitch / 2); c += 512) {
+      uint32_t lo[3], hi[3];
+      terms3(c < cols ? p[c] * scale : 0.f, lo);
+      terms3(c + 1 < cols ? p[c + 1] * scale : 0.f, hi);
+#pragma unroll
+      for (int i = 0; i < 3; ++i) d[i * (plane / 4) + c / 2] = lo[i] | hi[i] << 16;
+    }
+  }
+}
+
+// Rows of `bytes` bytes to rows of `pitch` (a multiple of 16), zeros behind.
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u32x4* __restrict__ dst,
+                                                   int rows, int cols, uint32_t pitch) {
+  constexpr int kPer = 16 / (int)sizeof(T);
+  const uint32_t chunks = pitch / 16;
+  const uint64_t total = (uint64_t)rows * chunks;
+  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
+    const uint64_t row = t / chunks;
+    const int c0 = (int)(t - row * chunks) * kPer;
+    const T* p = src + row * cols;
+    u32x4 v = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const uint32_t b = c0 + i < cols ? (uint32_t)p[c0 + i] : 0u;
+      v[i * (int)sizeof(T) / 4] |= b << (8 * ((i * (int)sizeof(T)) & 3));
+    }
+    dst[t] = v;
+  }
+}
+
+// dg = grad f_g(g, u) and du = grad f_u(g, u) of [rows][cols] values as BF16 planes
+// [terms][rows][2 half]: dg at columns [0, cols), du at [half, half + cols), zeros in the
+// rest; half is a multiple of 8.  One term rounds to BF16, three keep all 24 bits.
+__device__ __forceinline__ float widen(uint16_t b) { return bf16_bits_to_f32(b); }
+__device__ __forceinline__ float widen(float f) { return f; }
+
+template <typename T, int TERMS>
+__global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, const T* __restrict__ u,
+                                                    const T* __restrict__ grad,
+                                                    uint16_t* __restrict__ planes, int rows,
+                                                    int cols, int half, int act) {
+  const uint64_t plane = (uint64_t)rows * 2 * half;
+  const uint64_t total = (uint64_t)rows * half;
+  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
+    const uint64_t row = t / (uint32_t)half;
+    const int c = (int)(t - row * (uint32_t)half);
+    float dg = 0.f, du = 0.f;
+    if (c < cols) {
+      const uint64_t at = row * cols + c;
+      const float gv = widen(g[at]), uv = widen(u[at]), d = widen(grad[at]);
+      const float sig = 1.0f / (1.0f + expf(-gv));
+      if (act == K3_ACT_SILU) {
+        dg = d * uv * (sig * (1.0f + gv * (1.0f - sig)));
+        du = d * (gv * sig);
+      } else {
+        const float a = tanhf(gv / 4.0f), b = tanhf(uv / 25.0f);
+        dg = d * (25.0f * b) * ((1.0f - a * a) * sig + 4.0f * a * (sig * (1.0f - sig)));
+        du = d * (4.0f * a * sig) * (1.0f - b * b);
+      }
+    }
+    uint16_t* o = planes + row * 2 * half + c;
+    uint32_t tg[3], tu[3];
+    terms3(dg, tg);
+    terms3(du, tu);
+#pragma unroll
+    for (int i = 0; i < TERMS; ++i) {
+      o[i * plane] = (uint16_t)tg[i];
+      o[i * plane + half] = (uint16_t)tu[i];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ host
+bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
+uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
+uint32_t round_up(uint32_t v, uint32_t to) { return (v + to - 1) / to * to; }
+
+// Scratch memory in the order of its taking.
+struct Scratch {
+  uint8_t* base;
+  uint64_t used = 0;
+  explicit Scratch(void* p) : base(static_cast<uint8_t*>(p)) {}
+  uint8_t* take(uint64_t bytes) {
+    uint8_t* p = base ? base + used : nullptr;
+    used += align256(bytes);
+    return p;
+  }
+};
+
+unsigned grid_for(uint64_t threads) {
+  return (unsigned)std::min<uint64_t>((threads + 255) / 256, 1u << 16);
+}
+
+int launched_or(TimedLaunch& tl, const char* what) {
+  const hipError_t err = hipGetLastError();
+  if (err == hipSuccess) return K3_SPINE_OK;
+  tl.failed();
+  return spine_fail(K3_SPINE_E_RUNTIME, "%s: %s", what, hipGetErrorString(err));
+}
+
+int pack_rows(const void* src, void* dst, int elem, int rows, int cols, uint32_t pitch,
+              hipStream_t st) {
+  TimedLaunch tl(KC_SPLIT, st);
+  const unsigned grid = grid_for((uint64_t)rows * (pitch / 16));
+  if (elem == 2)
+    launch_timed(tl, k_pack_rows<uint16_t>, dim3(grid), dim3(256), 0, st,
+                 static_cast<const uint16_t*>(src), static_cast<u32x4*>(dst), rows, cols, pitch);
+  else
+    launch_timed(tl, k_pack_rows<uint8_t>, dim3(grid), dim3(256), 0, st,
+                 static_cast<const uint8_t*>(src), static_cast<u32x4*>(dst), rows, cols, pitch);
+  return launched_or(tl, "dense operand layout");
+}
+
+int split_rows(const void* x, void* planes, float* xs, int rows, int cols, uint32_t pitch,
+               hipStream_t st) {
+  TimedLaunch tl(KC_SPLIT, st);
+  launch_timed(tl, k_split_rows, dim3((unsigned)std::min(rows, 1 << 16)), dim3(256), 0, st,
+               static_cast<const float*>(x), static_cast<uint8_t*>(planes), xs, rows, cols, pitch);
+  return launched_or(tl, "dense activation terms");
+}
+
+// A matrix as an operand: in place where its rows are whole 16-byte pieces, else a
+// copy of it with rows that are.
+struct Matrix {
+  const void* src;
+  int elem, rows, cols;
+  uint32_t pitch;
+  uint8_t* copy = nullptr;  // scratch of the copy
+  bool copied;
+  Matrix(const void* p, int elem_, int rows_, int cols_, Scratch& s)
+      : src(p), elem(elem_), rows(rows_), cols(cols_) {
+    pitch = round_up((uint32_t)cols * elem, 16);
+    copied = pitch != (uint32_t)cols * elem || !aligned16(p);
+    if (copied) copy = s.take((uint64_t)rows * pitch);
+  }
+  const uint8_t* data() const { return copied ? copy : static_cast<const uint8_t*>(src); }
+  int fill(hipStream_t st) const {
+    return copied ? pack_rows(src, copy, elem, rows, cols, pitch, st) : K3_SPINE_OK;
+  }
+};
+
+// Activation rows as operand planes: bf16 rows as a Matrix, fp32 rows split.
+struct Activation {
+  const void* src;
+  bool f32;
+  int rows, cols;
+  uint32_t pitch;
+  uint8_t* planes = nullptr;
+  float* xs = nullptr;
+  bool copied = false;
+  Activation(const void* p, int dtype, int rows_, int cols_, bool scaled, Scratch& s)
+      : src(p), f32(dtype == K3_DTYPE_F32), rows(rows_), cols(cols_) {
+    pitch = round_up((uint32_t)cols * 2, 16);
+    if (f32) {
+      planes = s.take(3ull * rows * pitch);
+      if (scaled) xs = reinterpret_cast<float*>(s.take(4ull * rows));
+    } else {
+      copied = pitch != (uint32_t)cols * 2 || !aligned16(p);
+      if (copied) planes = s.take((uint64_t)rows * pitch);
+    }
+  }
+  int terms() const { return f32 ? 3 : 1; }
+  const uint8_t* plane(int t) const {
+    if (!f32 && !copied) return static_cast<const uint8_t*>(src);
+    return planes + (uint64_t)t * rows * pitch;
+  }
+  int fill(hipStream_t st) const {
+    if (f32) return split_rows(src, planes, xs, rows, cols, pitch, st);
+    return copied ? pack_rows(src, planes, 2, rows, cols, pitch, st) : K3_SPINE_OK;
+  }
+};
+
+// Tiles and the split of K.
+struct Plan {
+  bool large;
+  int tiles_n, tiles_m, splits, per, pitch;
+  float* part;
+};
+
+constexpr int kLargeN = 256, kLargeM = 256, kSmallN = 128, kSmallM = 128;
+
+Plan plan_product(int n, int m, int steps, bool glu, Scratch& s) {
+  const int cus = 256;
+  const int cols = glu ? (int)round_up((uint32_t)n, 16) * 2 : n;
+  Plan p{};
+  auto tiles = [&](int bn, int bm) {
+    return (int64_t)((cols + bn - 1) / bn) * ((m + bm - 1) / bm);
+  };
+  p.large = tiles(kLargeN, kLargeM) >= 192;
+  const int bn = p.large ? kLargeN : kSmallN, bm = p.large ? kLargeM : kSmallM;
+  p.tiles_n = (cols + bn - 1) / bn;
+  p.tiles_m = (m + bm - 1) / bm;
+  const int64_t slots = p.large ? cus : 2 * cus;
+  const int64_t t = tiles(bn, bm);
+  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(t, 1), steps / 8));
+  p.per = (int)((steps + splits - 1) / splits);
+  p.splits = (steps + p.per - 1) / p.per;
+  p.pitch = (int)round_up((uint32_t)cols, 4);
+  if (p.splits > 1)
+    p.part = reinterpret_cast<float*>(s.take(4ull * p.splits * m * p.pitch));
+  else
+    p.part = nullptr;
+  return p;
+}
+
+template <int WL, int XL, int EPI>
+int product(GemmArgs a, const Epilogue& e, const Plan& p, const char* what, hipStream_t st) {
+  a.tiles_n = p.tiles_n;
+  a.tiles_m = p.tiles_m;
+  a.splits = p.splits;
+  a.per = p.per;
+  const uint64_t tiles = (uint64_t)p.tiles_n * p.tiles_m;
+  if (tiles > UINT32_MAX / 512 || p.splits > 65535)
+    return spine_fail(K3_SPINE_E_INVALID, "%s: too many output tiles", what);
+  {
+    TimedLaunch tl(KC_SPINE_MFMA, st);
+    const dim3 grid((unsigned)tiles, (unsigned)p.splits);
+    float* part = p.splits > 1 ? p.part : nullptr;
+    if (p.large)
+      launch_timed(tl, (k_gemm<kLargeN, kLargeM, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e,
+                   part, p.pitch);
+    else
+      launch_timed(tl, (k_gemm<kSmallN, kSmallM, 2, 2, WL, XL, EPI>), grid, dim3(256), 0, st, a, e,
+                   part, p.pitch);
+    const int rc = launched_or(tl, what);
+    if (rc != K3_SPINE_OK) return rc;
+  }
+  if (p.splits == 1) return K3_SPINE_OK;
+  TimedLaunch tl(KC_COMBINE, st);
+  launch_timed(tl, k_gemm_join<EPI>, dim3(grid_for((uint64_t)e.m * ((e.n + 3) / 4))), dim3(256), 0,
+               st, e, p.part, p.splits, p.pitch);
+  return launched_or(tl, what);
+}
+
+int steps_of(int k) { return (k + kStep - 1) / kStep; }
+
+bool vec_ok(int n, int out_elem, std::initializer_list<const void*> ptrs) {
+  if (n % 4 != 0) return false;
+  for (const void* p : ptrs)
+    if (((uintptr_t)p & 15u) != 0) return false;
+  (void)out_elem;
+  return true;
+}
+
+struct LinearCall {
+  Scratch s;
+  Matrix w;
+  Activation x;
+  Plan p;
+  LinearCall(const K3HipLinearV1& op, void* ws)
+      : s(ws),
+        w(op.weights, op.matrix_kind == K3_SPINE_MATRIX_INT8 ? 1 : 2, (int)op.rows,
+          (int)op.columns, s),
+        x(op.x, (int)op.x_dtype, (int)op.positions, (int)op.columns, true, s),
+        p(plan_product((int)op.rows, (int)op.positions, x.terms() * steps_of((int)op.columns),
+                       false, s)) {}
+};
+
+struct GatedCall {
+  Scratch s;
+  Matrix g, u;
+  Activation x;
+  Plan p;
+  GatedCall(const K3HipGatedV1& op, void* ws)
+      : s(ws),
+        g(op.gate, op.matrix_kind == K3_SPINE_MATRIX_INT8 ? 1 : 2, (int)op.rows, (int)op.columns,
+          s),
+        u(op.up, g.elem, g.rows, g.cols, s),
+        x(op.x, (int)op.x_dtype, (int)op.positions, (int)op.columns, true, s),
+        p(plan_product((int)op.rows, (int)op.positions, x.terms() * steps_of((int)op.columns),
+                       true, s)) {}
+};
+
+// The products of the gradient: d_x over the 2 terms() segments of (dg, gate) and
+// (du, up), and both weight gradients as one product of 2 half rows.
+struct GradCall {
+  Scratch s;
+  Matrix g, u;
+  Activation x;
+  int half, terms;
+  uint16_t* planes;
+  Plan px, pw;
+  GradCall(const K3HipGatedGradV1& op, void* ws)
+      : s(ws),
+        g(op.gate, 2, (int)op.rows, (int)op.columns, s),
+        u(op.up, 2, (int)op.rows, (int)op.columns, s),
+        x(op.x, (int)op.dtype, (int)op.positions, (int)op.columns, false, s),
+        half((int)round_up(op.rows, 8)),
+        terms(x.terms()),
+        planes(reinterpret_cast<uint16_t*>(s.take(4ull * terms * op.positions * half))),
+        px(plan_product((int)op.columns, (int)op.positions,
+                        2 * terms * steps_of((int)op.rows), false, s)),
+        pw(plan_product((int)op.columns, 2 * half,
+                        (terms == 3 ? 6 : 1) * steps_of((int)op.positions), false, s)) {}
+};
+
+}  // namespace
+
+uint64_t dense_linear_workspace(const K3HipLinearV1& op) {
+  return std::max<uint64_t>(256, LinearCall(op, nullptr).s.used);
+}
+uint64_t dense_gated_workspace(const K3HipGatedV1& op) {
+  return std::max<uint64_t>(256, GatedCall(op, nullptr).s.used);
+}
+uint64_t dense_gated_grad_workspace(const K3HipGatedGradV1& op) {
+  return std::max<uint64_t>(256, GradCall(op, nullptr).s.used);
+}
+
+int dense_linear(const K3HipLinearV1& op, void* ws, hipStream_t st) {
+  const LinearCall c(op, ws);
+  int rc = c.w.fill(st);
+  if (rc == K3_SPINE_OK) rc = c.x.fill(st);
+  if (rc != K3_SPINE_OK) return rc;
+  const bool int8 = op.matrix_kind == K3_SPINE_MATRIX_INT8;
+  GemmArgs a{};
+  a.segments = c.x.terms();
+  for (int t = 0; t < a.segments; ++t) {
+    a.w[t] = c.w.data();
+    a.x[t] = c.x.plane(a.segments - 1 - t);  // the small terms first
+  }
+  a.n = (int)op.rows;
+  a.m = (int)op.positions;
+  a.k = (int)op.columns;
+  a.ldw = c.w.pitch;
+  a.kw = (int)(c.w.pitch / c.w.elem);
+  a.ldx = c.x.pitch;
+  a.kx = (int)(c.x.pitch / 2);
+  Epilogue e{};
+  e.rs = int8 ? op.row_scales : nullptr;
+  e.bias = op.bias;
+  e.xs = c.x.xs;
+  e.res = op.residual;
+  e.out = op.out;
+  e.n = a.n;
+  e.m = a.m;
+  e.act = (int)op.activation;
+  e.bf16 = op.out_dtype == K3_DTYPE_BF16;
+  e.vec = vec_ok(a.n, 0, {e.rs, op.bias, op.residual, op.out});
+  return int8 ? product<L_INT8, L_KMAJOR, EPI_LINEAR>(a, e, c.p, "linear", st)
+              : product<L_KMAJOR, L_KMAJOR, EPI_LINEAR>(a, e, c.p, "linear", st);
+}
+
+int dense_gated(const K3HipGatedV1& op, void* ws, hipStream_t st) {
+  const GatedCall c(op, ws);
+  int rc = c.g.fill(st);
+  if (rc == K3_SPINE_OK) rc = c.u.fill(st);
+  if (rc == K3_SPINE_OK) rc = c.x.fill(st);
+  if (rc != K3_SPINE_OK) return rc;
+  const bool int8 = op.matrix_kind == K3_SPINE_MATRIX_INT8;
+  GemmArgs a{};
+  a.segments = c.x.terms();
+  for (int t = 0; t < a.segments; ++t) {
+    a.w[t] = c.g.data();
+    a.w2[t] = c.u.data();
+    a.x[t] = c.x.plane(a.segments - 1 - t);
+  }
+  a.n = (int)op.rows;
+  a.m = (int)op.positions;
+  a.k = (int)op.columns;
+  a.ldw = c.g.pitch;
+  a.kw = (int)(c.g.pitch / c.g.elem);
+  a.ldx = c.x.pitch;
+  a.kx = (int)(c.x.pitch / 2);
+  Epilogue e{};
+  e.rs = int8 ? op.gate_scales : nullptr;
+  e.rs2 = int8 ? op.up_scales : nullptr;
+  e.xs = c.x.xs;
+  e.out = op.out;
+  e.out1 = op.out_gate;
+  e.out2 = op.out_up;
+  e.n = a.n;
+  e.m = a.m;
+  e.act = (int)op.activation;
+  e.bf16 = op.out_dtype == K3_DTYPE_BF16;
+  e.vec = vec_ok(a.n, 0, {e.rs, e.rs2, op.out, op.out_gate, op.out_up});
+  return int8 ? product<L_INT8, L_KMAJOR, EPI_GLU>(a, e, c.p, "gated feed-forward", st)
+              : product<L_KMAJOR, L_KMAJOR, EPI_GLU>(a, e, c.p, "gated feed-forward", st);
+}
+
+int dense_gated_grad(const K3HipGatedGradV1& op, void* ws, hipStream_t st) {
+  const GradCall c(op, ws);
+  const char* what = "gated feed-forward gradient";
+  const bool f32 = op.dtype == K3_DTYPE_F32;
+  const int P = (int)op.positions, S = (int)op.rows, H = (int)op.columns;
+  int rc = c.g.fill(st);
+  if (rc == K3_SPINE_OK) rc = c.u.fill(st);
+  if (rc == K3_SPINE_OK) rc = c.x.fill(st);
+  if (rc != K3_SPINE_OK) return rc;
+  {
+    TimedLaunch tl(KC_ACTIVATE, st);
+    const dim3 grid(grid_for((uint64_t)P * c.half));
+    if (f32)
+      launch_timed(tl, (k_gated_grad<float, 3>), grid, dim3(256), 0, st,
+                   static_cast<const float*>(op.g), static_cast<const float*>(op.u),
+                   static_cast<const float*>(op.grad), c.planes, P, S, c.half, (int)op.activation);
+    else
+      launch_timed(tl, (k_gated_grad<uint16_t, 1>), grid, dim3(256), 0, st,
+                   static_cast<const uint16_t*>(op.g), static_cast<const uint16_t*>(op.u),
+                   static_cast<const uint16_t*>(op.grad), c.planes, P, S, c.half,
+                   (int)op.activation);
+    if ((rc = launched_or(tl, what)) != K3_SPINE_OK) return rc;
+  }
+  const uint32_t ldd = 4u * (uint32_t)c.half;  // bytes of a row of dg and du
+  auto plane = [&](int t, int which) {
+    return reinterpret_cast<const uint8_t*>(c.planes) + (uint64_t)t * P * ldd + 2ull * which * c.half;
+  };
+  GemmArgs a{};
+  for (int t = c.terms - 1; t >= 0; --t)
+    for (int which = 0; which < 2; ++which) {
+      a.w[a.segments] = which ? c.u.data() : c.g.data();
+      a.x[a.segments] = plane(t, which);
+      ++a.segments;
+    }
+  a.n = H;
+  a.m = P;
+  a.k = S;
+  a.kw = S;
+  a.kx = c.half;
+  a.ldw = c.g.pitch;
+  a.ldx = ldd;
+  Epilogue e{};
+  e.out = op.d_x;
+  e.n = H;
+  e.m = P;
+  e.bf16 = !f32;
+  e.vec = vec_ok(H, 0, {op.d_x});
+  rc = product<L_NMAJOR, L_KMAJOR, EPI_GRAD>(a, e, c.px, what, st);
+  if (rc != K3_SPINE_OK) return rc;
+
+  // term pairs (of dg / du, of x), the small products first
+  static const int kPairs[6][2] = {{0, 2}, {2, 0}, {1, 1}, {1, 0}, {0, 1}, {0, 0}};
+  GemmArgs b{};
+  b.segments = f32 ? 6 : 1;
+  for (int i = 0; i < b.segments; ++i) {
+    const int* t = kPairs[f32 ? i : 5];
+    b.x[i] = plane(t[0], 0);
+    b.w[i] = c.x.plane(t[1]);
+  }
+  b.n = H;
+  b.m = 2 * c.half;
+  b.k = b.kw = b.kx = P;
+  b.ldw = c.x.pitch;
+  b.ldx = ldd;
+  Epilogue f{};
+  f.out = op.d_gate;
+  f.out1 = op.d_up;
+  f.n = H;
+  f.m = 2 * c.half;
+  f.half = c.half;
+  f.valid = S;
+  f.bf16 = !f32;
+  f.vec = vec_ok(H, 0, {op.d_gate, op.d_up});
+  return product<L_NMAJOR, L_NMAJOR, EPI_GRAD>(b, f, c.pw, what, st);
+}
+
+}  // namespace k3

@@ -1,0 +1,281 @@
+// Tiled matrix-core products D[m, n] = sum_k W(n, k) X(m, k) for many positions:
+// the device core of the dense layers (k3_dense.hip).  Both operands are BF16 planes
+// in memory (an fp32 operand is several planes, see below; int8 weights are widened
+// in registers), sums are fp32.
+//
+// Segments.  A product is a list of up to six segments, each a pair of planes over the
+// same K: the three BF16 terms of an fp32 activation against one matrix, the six
+// leading term pairs of two fp32 operands, or the gate and the up half of a gradient.
+// All segments of an output meet in the same accumulators, so an fp32 product costs
+// three (or six) BF16 products and no pass over the output in between.
+//
+// Tile.  A workgroup computes BN x BM outputs in K steps of 64 through two LDS buffers:
+// while one is multiplied the next step comes from memory straight into the other
+// (global_load_lds, 16 bytes per lane, no registers held).  One instruction of a wave
+// fills 1 KB of LDS in lane order, so the layout in LDS is chosen by which 16 bytes of
+// memory each lane asks for:
+//   KMAJOR  rows of 64 k (128 bytes), 16-byte chunk c of row r at slot c ^ (r % 8);
+//   INT8    rows of 64 k (64 bytes), chunk c at slot c ^ ((r / 2) % 4);
+//   NMAJOR  (the operand's k runs over memory rows) 64 k rows of BN (BM) values,
+//           32-byte chunk c of row k at slot c ^ nmajor_swizzle(k), read back through
+//           ds_read_b64_tr_b16, which hands 16 lanes the columns of 4 rows x 16 values.
+// The exclusive-ors spread each read of a wave over all banks.
+//
+// The k of an operand element is 16 g + 8 kk + e in a step (lane group g = lane / 16,
+// half kk, element e) instead of the matrix instruction's 32 kk + 8 g + e: any order
+// serves as long as both operands use it, and this one lets an int8 lane read its 16
+// values of both halves at once.
+//
+// The weight operand is the instruction's first, so a lane's four results are four
+// consecutive n of one m: 8 or 16 bytes of a row-major output.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "k3_device.h"
+
+namespace k3 {
+namespace gemm {
+
+enum { L_KMAJOR = 0, L_INT8 = 1, L_NMAJOR = 2 };
+
+constexpr int kStep = 64;      // k of a step
+constexpr int kMaxSegments = 6;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+struct GemmArgs {
+  const uint8_t* w[kMaxSegments];   // weight-side planes
+  const uint8_t* w2[kMaxSegments];  // GLU: the up matrix's (w is the gate's)
+  const uint8_t* x[kMaxSegments];   // position-side planes
+  int segments;
+  int n, m, k;         // n: of one matrix (GLU: outputs); k per segment
+  int kw, kx;          // k held by a KMAJOR / INT8 row in memory, whole chunks (>= k)
+  uint32_t ldw, ldx;   // bytes between rows
+  int tiles_n, tiles_m;
+  int splits, per;     // steps [z * per, ...) of all segments' for grid z
+};
+
+__device__ const u32x4 g_zero_chunk = {0u, 0u, 0u, 0u};
+
+// 16 bytes per lane from memory to LDS at base + 16 lane; base is wave-uniform.
+__device__ __forceinline__ void load_lds(const uint8_t* src, uint8_t* base) {
+  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+}
+
+template <int R>
+__device__ __forceinline__ int nmajor_swizzle(int k) {
+  return ((k & 3) | ((k >> 4 & 1) << 2)) & (R / 16 - 1);
+}
+
+// An operand's tile of R rows (n or m) x 64 k.
+template <int R, int L, int WAVES, bool kPairs>
+struct Tile {
+  static constexpr int kBytes = R * kStep * (L == L_INT8 ? 1 : 2);
+  static constexpr int kLoads = kBytes / 1024;                      // wave instructions
+  static constexpr int kPer = (kLoads + WAVES - 1) / WAVES;         // of one wave
+  static constexpr int kChunkK = L == L_INT8 ? 16 : 8;              // k of a 16-byte chunk
+  static constexpr int kRowLoads = R / 8;                           // NMAJOR: chunks of a k row
+  static_assert(kLoads * 1024 == kBytes, "whole instructions");
+
+  uint32_t off[kPer];  // lane offsets from the segment's (matrix's) base at k = 0
+
+  // rows: of the operand (n or m); r0: the tile's first.  With kPairs the tile's
+  // blocks of 16 rows alternate between the gate and the up matrix.
+  __device__ __forceinline__ void init(int wave, int lane, int r0, int rows, uint32_t ld) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = wave * kPer + i;
+      if constexpr (L == L_NMAJOR) {
+        const int kr = j * (64 / kRowLoads) + lane / kRowLoads;
+        const int pos = lane % kRowLoads;
+        const int c = (pos >> 1) ^ nmajor_swizzle<R>(kr);
+        // rows past the last chunk repeat the tile's first (never stored)
+        const int r = c * 16 + (pos & 1) * 8;
+        off[i] = (uint32_t)kr * ld + (uint32_t)(r0 + r < rows ? r : 0) * 2u;
+      } else {
+        const int per = L == L_INT8 ? 16 : 8;  // rows of an instruction
+        const int rl = j * per + lane / (64 / per);
+        const int r = kPairs ? (rl >> 5) * 16 + (rl & 15) : rl;
+        const int slot = lane % (64 / per);
+        const int c = L == L_INT8 ? slot ^ ((rl >> 1) & 3) : slot ^ (rl & 7);
+        off[i] = (uint32_t)min(r, rows - 1 - r0) * ld + 16u * c;
+      }
+    }
+  }
+
+  // Step at k0 from base (the operand's row r0, k = 0; NMAJOR: k = 0, column r0) to lds.
+  // k_end: k held by memory rows; tail steps read zeros past it.
+  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t* base2, int wave,
+                                       int lane, int k0, int k_end, uint32_t ld,
+                                       uint8_t* lds) const {
+    const bool tail = k0 + kStep > k_end;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = wave * kPer + i;
+      if (kLoads % WAVES != 0 && j >= kLoads) break;
+      const uint8_t* b = base;
+      if (kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2) b = base2;
+      b += L == L_NMAJOR ? (uint64_t)k0 * ld : (uint64_t)k0 * (L == L_INT8 ? 1 : 2);
+      const uint8_t* p = b + off[i];
+      if (tail) {
+        int k;
+        if constexpr (L == L_NMAJOR) {
+          k = k0 + j * (64 / kRowLoads) + lane / kRowLoads;
+        } else {
+          const int per = L == L_INT8 ? 16 : 8;
+          const int rl = j * per + lane / (64 / per);
+          const int slot = lane % (64 / per);
+          k = k0 + kChunkK * (L == L_INT8 ? slot ^ ((rl >> 1) & 3) : slot ^ (rl & 7));
+        }
+        if (k >= k_end) p = reinterpret_cast<const uint8_t*>(&g_zero_chunk);
+      }
+      load_lds(p, lds + 1024 * j);
+    }
+  }
+};
+
+__device__ __forceinline__ bf16x8 widen8(uint32_t a, uint32_t b) {
+  uint32_t p[4];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const uint32_t v = e ? b : a;
+    uint32_t f[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[i] = __float_as_uint((float)((int32_t)(v << (24 - 8 * i)) >> 24));
+    p[2 * e] = __builtin_amdgcn_perm(f[1], f[0], 0x07060302u);
+    p[2 * e + 1] = __builtin_amdgcn_perm(f[3], f[2], 0x07060302u);
+  }
+  return __builtin_bit_cast(bf16x8, u32x4{p[0], p[1], p[2], p[3]});
+}
+
+// Operand fragments: F blocks of 16 rows from row16 * 16 of the tile, both halves.
+template <int R, int L, int F>
+struct Frags {
+  bf16x8 v[2][F];
+
+  template <int kk>
+  __device__ __forceinline__ void read(const uint8_t* lds, int row16, int lane) {
+    const int i16 = lane & 15, g = lane >> 4;
+    if constexpr (L == L_KMAJOR) {
+      const uint8_t* p = lds + row16 * 2048 + i16 * 128 + (((2 * g + kk) ^ (i16 & 7)) << 4);
+#pragma unroll
+      for (int f = 0; f < F; ++f) v[kk][f] = *reinterpret_cast<const bf16x8*>(p + 2048 * f);
+    } else if constexpr (L == L_INT8) {
+      if constexpr (kk == 0) {
+        const uint8_t* p = lds + row16 * 1024 + i16 * 64 + ((g ^ ((i16 >> 1) & 3)) << 4);
+#pragma unroll
+        for (int f = 0; f < F; ++f) {
+          const u32x4 q = *reinterpret_cast<const u32x4*>(p + 1024 * f);
+          v[0][f] = widen8(q.x, q.y);
+          v[1][f] = widen8(q.z, q.w);
+        }
+      }
+    } else {
+      const int kr = 16 * g + 8 * kk + (i16 >> 2);  // and kr + 4: the same swizzle
+      const uint8_t* p = lds + kr * (2 * R) + (i16 & 3) * 8;
+      const int s = nmajor_swizzle<R>(kr);
+#pragma unroll
+      for (int f = 0; f < F; ++f) {
+        const uint8_t* q = p + (((row16 + f) ^ s) << 5);
+        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 8 * R));
+        const bf16x4 a = __builtin_bit_cast(bf16x4, lo), b = __builtin_bit_cast(bf16x4, hi);
+        v[kk][f] = bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      }
+    }
+  }
+};
+
+// Workgroup of tile t: the eight XCDs take contiguous runs of tiles, so that one L2
+// holds the panels that its workgroups share, and within the order a band of kBand
+// row panels is walked before the next column panel.
+constexpr int kXcds = 8;
+constexpr int kBand = 4;
+__device__ __forceinline__ void tile_of(int b, int tiles_n, int tiles_m, int* tn, int* tm) {
+  const int total = tiles_n * tiles_m;
+  const int q = total / kXcds, r = total % kXcds, x = b % kXcds;
+  const int t = x * q + min(x, r) + b / kXcds;
+  const int band = t / (kBand * tiles_n);
+  const int m0 = band * kBand, mh = min(kBand, tiles_m - m0);
+  const int in = t - m0 * tiles_n;
+  *tm = m0 + in % mh;
+  *tn = in / mh;
+}
+
+// The tile's sums: acc[fn][fm] of a wave, n = n0 + 16 fn + 4 (lane / 16) + i,
+// m = m0 + 16 fm + lane % 16 with the wave's n0, m0 below.
+template <int BN, int BM, int NWN, int NWM, int WL, int XL, bool kPairs>
+struct Core {
+  static constexpr int kWaves = NWN * NWM;
+  static constexpr int FN = BN / 16 / NWN, FM = BM / 16 / NWM;
+  typedef Tile<BN, WL, kWaves, kPairs> TW;
+  typedef Tile<BM, XL, kWaves, false> TX;
+  static constexpr int kBuffer = TW::kBytes + TX::kBytes;
+
+  __device__ static __forceinline__ void run(const GemmArgs& a, uint8_t* lds, int tn, int tm,
+                                             int split, f32x4 (&acc)[FN][FM]) {
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wn = wave % NWN, wm = wave / NWN;
+    const int rn = tn * (kPairs ? BN / 2 : BN), rm = tm * BM;
+    TW tw;
+    TX tx;
+    tw.init(wave, lane, rn, a.n, a.ldw);
+    tx.init(wave, lane, rm, a.m, a.ldx);
+    const uint64_t w0 = WL == L_NMAJOR ? (uint64_t)rn * 2 : (uint64_t)rn * a.ldw;
+    const uint64_t x0 = XL == L_NMAJOR ? (uint64_t)rm * 2 : (uint64_t)rm * a.ldx;
+    const int steps = (a.k + kStep - 1) / kStep;
+    const int s0 = split * a.per, s1 = min(s0 + a.per, steps * a.segments);
+
+#pragma unroll
+    for (int i = 0; i < FN; ++i)
+#pragma unroll
+      for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    int seg = s0 / steps, k0 = (s0 - seg * steps) * kStep;
+    auto load = [&](uint8_t* buf) {
+      tw.load(a.w[seg] + w0, kPairs ? a.w2[seg] + w0 : nullptr, wave, lane, k0, a.kw, a.ldw, buf);
+      tx.load(a.x[seg] + x0, nullptr, wave, lane, k0, a.kx, a.ldx, buf + TW::kBytes);
+      k0 += kStep;
+      if (k0 >= a.k) {
+        k0 = 0;
+        ++seg;
+      }
+    };
+    if (s0 < s1) load(lds);
+    for (int s = s0; s < s1; ++s) {
+      uint8_t* cur = lds + ((s - s0) & 1) * kBuffer;
+      uint8_t* nxt = lds + ((s - s0 + 1) & 1) * kBuffer;
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the step is there
+      __syncthreads();                     // everybody's is, and nxt is no longer read
+      if (s + 1 < s1) load(nxt);
+      Frags<BN, WL, FN> fw;
+      Frags<BM, XL, FM> fx;
+      fw.template read<0>(cur, wn * FN, lane);
+      fx.template read<0>(cur + TW::kBytes, wm * FM, lane);
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+          acc[i][j] =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw.v[0][i], fx.v[0][j], acc[i][j], 0, 0, 0);
+      fw.template read<1>(cur, wn * FN, lane);
+      fx.template read<1>(cur + TW::kBytes, wm * FM, lane);
+#pragma unroll
+      for (int i = 0; i < FN; ++i)
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+          acc[i][j] =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw.v[1][i], fx.v[1][j], acc[i][j], 0, 0, 0);
+    }
+  }
+};
+
+}  // namespace gemm
+}  // namespace k3
