@@ -1,5 +1,5 @@
-"""ctypes binding of libk3hipmoe.so (the C ABI in include/k3_hip_moe_abi.h and
-include/k3_hip_spine_abi.h).
+"""ctypes binding of libk3hipmoe.so (the C ABI in include/k3_hip_moe_abi.h,
+k3_hip_spine_abi.h, k3_hip_dense_abi.h and k3_hip_sample_abi.h).
 
 The library is loaded after torch so that it binds to the HIP runtime torch
 already mapped (both carry the SONAME libamdhip64.so.7); loading fails loudly if
@@ -167,6 +167,27 @@ class K3HipGatedGradV1(C.Structure):
     ]
 
 
+class K3HipSampleV1(C.Structure):
+    _fields_ = [
+        ("abi_version", C.c_uint32),
+        ("struct_bytes", C.c_uint32),
+        ("logits_dtype", C.c_uint32),
+        ("rows", C.c_uint32),
+        ("vocabulary", C.c_uint32),
+        ("reserved", C.c_uint32),
+        ("logits", C.c_void_p),
+        ("u", C.c_void_p),
+        ("temperature", C.c_void_p),
+        ("top_k", C.c_void_p),
+        ("top_p", C.c_void_p),
+        ("min_p", C.c_void_p),
+        ("tokens", C.c_void_p),
+    ]
+
+
+K3_SAMPLE_ABI_V1 = 1
+K3_SAMPLE_MAX_ROWS = 32768
+K3_SAMPLE_MAX_VOCABULARY = 16777216
 K3_DENSE_ABI_V1 = 1
 K3_DENSE_MAX_EXTENT = 1048576
 K3_DENSE_ACT_NONE, K3_DENSE_ACT_SILU, K3_DENSE_ACT_GELU = 0, 1, 2
@@ -193,6 +214,7 @@ assert C.sizeof(K3HipCachePolicyV1) == 32
 
 assert C.sizeof(K3HipMoeSpineV1) == 144
 assert C.sizeof(K3HipLinearV1) == 88
+assert C.sizeof(K3HipSampleV1) == 80
 assert C.sizeof(K3HipGatedV1) == 104
 assert C.sizeof(K3HipGatedGradV1) == 104
 assert C.sizeof(K3HipKernelTimingV1) == 64
@@ -290,6 +312,9 @@ SIGNATURES = {
     "k3_hip_gated_ffn": (_i32, [C.POINTER(K3HipGatedV1), _vp, _u64, _vp]),
     "k3_hip_gated_ffn_grad_workspace_bytes": (_u64, [C.POINTER(K3HipGatedGradV1)]),
     "k3_hip_gated_ffn_grad": (_i32, [C.POINTER(K3HipGatedGradV1), _vp, _u64, _vp]),
+    # include/k3_hip_sample_abi.h
+    "k3_hip_sample_workspace_bytes": (_u64, [C.POINTER(K3HipSampleV1)]),
+    "k3_hip_sample": (_i32, [C.POINTER(K3HipSampleV1), _vp, _u64, _vp]),
 }
 
 _LIB: C.CDLL | None = None

@@ -50,7 +50,7 @@ CXX_FLAGS = [
     "-Wno-unused-parameter",
 ]
 KERNEL_SOURCES = ["k3_kernels.hip", "k3_verify_mfma.hip", "k3_spine.hip", "k3_skinny.hip",
-                  "k3_noalloc.hip", "k3_dense.hip"]
+                  "k3_noalloc.hip", "k3_dense.hip", "k3_sample.hip"]
 HOST_SOURCES = ["k3_abi.cpp", "k3_cache.cpp", "k3_timing.cpp", "k3_spine_abi.cpp",
                 "k3_dense_abi.cpp"]
 
