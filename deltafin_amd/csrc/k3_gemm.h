@@ -14,8 +14,8 @@
 // (global_load_lds, 16 bytes per lane, no registers held).  One instruction of a wave
 // fills 1 KB of LDS in lane order, so the layout in LDS is chosen by which 16 bytes of
 // memory each lane asks for:
-//   KMAJOR  rows of 64 k (128 bytes), 16-byte chunk c of row r at slot c ^ (r % 8);
-//   INT8    rows of 64 k (64 bytes), chunk c at slot c ^ ((r / 2) % 4);
+//   KMAJOR  rows of 64 k (128 bytes), 16-byte chunk c of row r at slot c ^ kmajor_swizzle(r);
+//   INT8    rows of 64 k (64 bytes), chunk c at slot c ^ int8_swizzle(r);
 //   NMAJOR  (the operand's k runs over memory rows) 64 k rows of BN (BM) values,
 //           32-byte chunk c of row k at slot c ^ nmajor_swizzle(k), read back through
 //           ds_read_b64_tr_b16, which hands 16 lanes the columns of 4 rows x 16 values.
@@ -62,9 +62,41 @@ struct GemmArgs {
 
 __device__ const u32x4 g_zero_chunk = {0u, 0u, 0u, 0u};
 
-// 16 bytes per lane from memory to LDS at base + 16 lane; base is wave-uniform.
-__device__ __forceinline__ void load_lds(const uint8_t* src, uint8_t* base) {
-  __builtin_amdgcn_global_load_lds(src, (__attribute__((address_space(3))) void*)base, 16, 0, 0);
+// 16 bytes per lane from memory to LDS at `lds` + 16 lane (wave-uniform, as is `base`).  In
+// assembly for its address form, a scalar base and a 32-bit lane offset: through the
+// builtin every load took a 64-bit lane address of its own, whose sums and register pairs
+// cost the large tile its spare registers.  It writes no register but m0, which the
+// compiler holds nothing in (it sets m0 right ahead of what reads it); vmcnt ends it.
+__device__ __forceinline__ void load_lds(const uint8_t* base, uint32_t offset, uint32_t lds) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+      :
+      : "s"(lds), "v"(offset), "s"(base)
+      : "memory");
+}
+__device__ __forceinline__ void load_lds(const uint8_t* lane_address, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(lds), "v"(lane_address)
+               : "memory");
+}
+// All of this wave's loads have landed, then everybody's.
+__device__ __forceinline__ void landed() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  __syncthreads();
+}
+
+// A 16-byte read of a wave runs as four passes of 16 lanes, lanes 0-3, 12-15 and 20-27
+// the first: 16 different rows of the 16, eight of them in one lane group's chunk and
+// eight in the next one's.  These orders put such a pass on all 64 banks (counted: with
+// c ^ (r % 8) or c ^ (r / 2 % 8) every read took twice its cycles).
+__device__ __forceinline__ int kmajor_swizzle(int r) {
+  const int q = (r >> 1) & 7;
+  return q ^ ((q & 2) << 1);
+}
+__device__ __forceinline__ int int8_swizzle(int r) {
+  const int t = (r >> 2) & 3;
+  return (t >> 1) | (((t ^ (t >> 1)) & 1) << 1);
 }
 
 template <int R>
@@ -102,39 +134,44 @@ struct Tile {
         const int rl = j * per + lane / (64 / per);
         const int r = kPairs ? (rl >> 5) * 16 + (rl & 15) : rl;
         const int slot = lane % (64 / per);
-        const int c = L == L_INT8 ? slot ^ ((rl >> 1) & 3) : slot ^ (rl & 7);
+        const int c = L == L_INT8 ? slot ^ int8_swizzle(rl) : slot ^ kmajor_swizzle(rl);
         off[i] = (uint32_t)min(r, rows - 1 - r0) * ld + 16u * c;
       }
     }
   }
 
-  // Step at k0 from base (the operand's row r0, k = 0; NMAJOR: k = 0, column r0) to lds.
-  // k_end: k held by memory rows; tail steps read zeros past it.
+  // The step at base (the operand's row r0, k = k0; NMAJOR: k = k0, column r0; base2 in the
+  // up matrix) to lds.
   __device__ __forceinline__ void load(const uint8_t* base, const uint8_t* base2, int wave,
-                                       int lane, int k0, int k_end, uint32_t ld,
-                                       uint8_t* lds) const {
-    const bool tail = k0 + kStep > k_end;
+                                       uint32_t lds) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int j = wave * kPer + i;
       if (kLoads % WAVES != 0 && j >= kLoads) break;
-      const uint8_t* b = base;
-      if (kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2) b = base2;
-      b += L == L_NMAJOR ? (uint64_t)k0 * ld : (uint64_t)k0 * (L == L_INT8 ? 1 : 2);
-      const uint8_t* p = b + off[i];
-      if (tail) {
-        int k;
-        if constexpr (L == L_NMAJOR) {
-          k = k0 + j * (64 / kRowLoads) + lane / kRowLoads;
-        } else {
-          const int per = L == L_INT8 ? 16 : 8;
-          const int rl = j * per + lane / (64 / per);
-          const int slot = lane % (64 / per);
-          k = k0 + kChunkK * (L == L_INT8 ? slot ^ ((rl >> 1) & 3) : slot ^ (rl & 7));
-        }
-        if (k >= k_end) p = reinterpret_cast<const uint8_t*>(&g_zero_chunk);
+      const uint8_t* b = kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base;
+      load_lds(b, off[i], lds + 1024 * j);
+    }
+  }
+
+  // The same where only `left` < 64 k of the step exist in memory: zeros past them.
+  __device__ __forceinline__ void load_tail(const uint8_t* base, const uint8_t* base2, int wave,
+                                            int lane, int left, uint32_t lds) const {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int j = wave * kPer + i;
+      if (kLoads % WAVES != 0 && j >= kLoads) break;
+      const uint8_t* b = kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base;
+      int k;
+      if constexpr (L == L_NMAJOR) {
+        k = j * (64 / kRowLoads) + lane / kRowLoads;
+      } else {
+        const int per = L == L_INT8 ? 16 : 8;
+        const int rl = j * per + lane / (64 / per);
+        const int slot = lane % (64 / per);
+        k = kChunkK * (L == L_INT8 ? slot ^ int8_swizzle(rl) : slot ^ kmajor_swizzle(rl));
       }
-      load_lds(p, lds + 1024 * j);
+      load_lds(k < left ? b + off[i] : reinterpret_cast<const uint8_t*>(&g_zero_chunk),
+               lds + 1024 * j);
     }
   }
 };
@@ -153,41 +190,49 @@ __device__ __forceinline__ bf16x8 widen8(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(bf16x8, u32x4{p[0], p[1], p[2], p[3]});
 }
 
-// Operand fragments: F blocks of 16 rows from row16 * 16 of the tile, both halves.
+// Operand fragments: F blocks of 16 rows from row16 * 16 of the tile, both halves.  int8
+// values are read with the first half and widened by widen() ahead of each half's use.
 template <int R, int L, int F>
 struct Frags {
   bf16x8 v[2][F];
+  u32x4 raw[L == L_INT8 ? F : 1];  // both halves' int8 values as read
 
   template <int kk>
   __device__ __forceinline__ void read(const uint8_t* lds, int row16, int lane) {
     const int i16 = lane & 15, g = lane >> 4;
     if constexpr (L == L_KMAJOR) {
-      const uint8_t* p = lds + row16 * 2048 + i16 * 128 + (((2 * g + kk) ^ (i16 & 7)) << 4);
+      const uint8_t* p = lds + row16 * 2048 + i16 * 128 + (((2 * g + kk) ^ kmajor_swizzle(i16)) << 4);
 #pragma unroll
       for (int f = 0; f < F; ++f) v[kk][f] = *reinterpret_cast<const bf16x8*>(p + 2048 * f);
     } else if constexpr (L == L_INT8) {
       if constexpr (kk == 0) {
-        const uint8_t* p = lds + row16 * 1024 + i16 * 64 + ((g ^ ((i16 >> 1) & 3)) << 4);
+        const uint8_t* p = lds + row16 * 1024 + i16 * 64 + ((g ^ int8_swizzle(i16)) << 4);
 #pragma unroll
-        for (int f = 0; f < F; ++f) {
-          const u32x4 q = *reinterpret_cast<const u32x4*>(p + 1024 * f);
-          v[0][f] = widen8(q.x, q.y);
-          v[1][f] = widen8(q.z, q.w);
-        }
+        for (int f = 0; f < F; ++f) raw[f] = *reinterpret_cast<const u32x4*>(p + 1024 * f);
       }
     } else {
       const int kr = 16 * g + 8 * kk + (i16 >> 2);  // and kr + 4: the same swizzle
-      const uint8_t* p = lds + kr * (2 * R) + (i16 & 3) * 8;
-      const int s = nmajor_swizzle<R>(kr);
+      // the chunk's place; opaque, so that the F exclusive-ors stay here instead of in F
+      // registers across the loop (which spilled)
+      uint32_t at = kr * (2 * R) + (i16 & 3) * 8 + ((row16 ^ nmajor_swizzle<R>(kr)) << 5);
+      asm volatile("" : "+v"(at));
 #pragma unroll
       for (int f = 0; f < F; ++f) {
-        const uint8_t* q = p + (((row16 + f) ^ s) << 5);
+        const uint8_t* q = lds + (at ^ (f << 5));
         typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
         const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
         const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 8 * R));
         const bf16x4 a = __builtin_bit_cast(bf16x4, lo), b = __builtin_bit_cast(bf16x4, hi);
         v[kk][f] = bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
       }
+    }
+  }
+
+  template <int kk>
+  __device__ __forceinline__ void widen() {
+    if constexpr (L == L_INT8) {
+#pragma unroll
+      for (int f = 0; f < F; ++f) v[kk][f] = widen8(raw[f][2 * kk], raw[f][2 * kk + 1]);
     }
   }
 };
@@ -238,41 +283,76 @@ struct Core {
 #pragma unroll
       for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
+    // where the next step comes from: pointers that advance, read anew per segment
     int seg = s0 / steps, k0 = (s0 - seg * steps) * kStep;
-    auto load = [&](uint8_t* buf) {
-      tw.load(a.w[seg] + w0, kPairs ? a.w2[seg] + w0 : nullptr, wave, lane, k0, a.kw, a.ldw, buf);
-      tx.load(a.x[seg] + x0, nullptr, wave, lane, k0, a.kx, a.ldx, buf + TW::kBytes);
+    const uint64_t dw = WL == L_NMAJOR ? (uint64_t)kStep * a.ldw : kStep * (WL == L_INT8 ? 1 : 2);
+    const uint64_t dx = XL == L_NMAJOR ? (uint64_t)kStep * a.ldx : kStep * 2;
+    const uint8_t *pw = nullptr, *pu = nullptr, *px = nullptr;
+    auto open = [&](int step) {
+      pw = a.w[seg] + w0 + step * dw;
+      if constexpr (kPairs) pu = a.w2[seg] + w0 + step * dw;
+      px = a.x[seg] + x0 + step * dx;
+    };
+    auto load = [&](uint32_t buf) {
+      if (__builtin_expect(k0 + kStep > a.kw, 0))
+        tw.load_tail(pw, pu, wave, lane, a.kw - k0, buf);
+      else
+        tw.load(pw, pu, wave, buf);
+      if (__builtin_expect(k0 + kStep > a.kx, 0))
+        tx.load_tail(px, nullptr, wave, lane, a.kx - k0, buf + TW::kBytes);
+      else
+        tx.load(px, nullptr, wave, buf + TW::kBytes);
       k0 += kStep;
-      if (k0 >= a.k) {
+      pw += dw;
+      if constexpr (kPairs) pu += dw;
+      px += dx;
+      if (k0 >= a.k && ++seg < a.segments) {
         k0 = 0;
-        ++seg;
+        open(0);
       }
     };
-    if (s0 < s1) load(lds);
+    if (s0 >= s1) return;
+    Frags<BN, WL, FN> fw;
+    Frags<BM, XL, FM> fx;
+    auto multiply = [&](int kk) {
+#pragma unroll
+      for (int j = 0; j < FM; ++j)
+#pragma unroll
+        for (int i = 0; i < FN; ++i)
+          acc[i][j] =
+              __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw.v[kk][i], fx.v[kk][j], acc[i][j], 0, 0, 0);
+    };
+    open(k0 / kStep);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    load(lds0);
+    landed();
+    if (s0 + 1 < s1) load(lds0 + kBuffer);
+    fw.template read<0>(lds, wn * FN, lane);
+    fx.template read<0>(lds + TW::kBytes, wm * FM, lane);
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
     for (int s = s0; s < s1; ++s) {
       uint8_t* cur = lds + ((s - s0) & 1) * kBuffer;
       uint8_t* nxt = lds + ((s - s0 + 1) & 1) * kBuffer;
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's part of the step is there
-      __syncthreads();                     // everybody's is, and nxt is no longer read
-      if (s + 1 < s1) load(nxt);
-      Frags<BN, WL, FN> fw;
-      Frags<BM, XL, FM> fx;
-      fw.template read<0>(cur, wn * FN, lane);
-      fx.template read<0>(cur + TW::kBytes, wm * FM, lane);
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j)
-          acc[i][j] =
-              __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw.v[0][i], fx.v[0][j], acc[i][j], 0, 0, 0);
+      // the first half's products cover the reads of the second
       fw.template read<1>(cur, wn * FN, lane);
       fx.template read<1>(cur + TW::kBytes, wm * FM, lane);
-#pragma unroll
-      for (int i = 0; i < FN; ++i)
-#pragma unroll
-        for (int j = 0; j < FM; ++j)
-          acc[i][j] =
-              __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw.v[1][i], fx.v[1][j], acc[i][j], 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      fw.template widen<0>();
+      multiply(0);
+      fw.template widen<1>();
+      __builtin_amdgcn_sched_barrier(0);
+      // the next step has landed and nobody reads this one any more
+      landed();
+      if (s + 2 < s1) load(lds0 + ((s - s0) & 1) * kBuffer);
+      if (s + 1 < s1) {
+        fw.template read<0>(nxt, wn * FN, lane);
+        fx.template read<0>(nxt + TW::kBytes, wm * FM, lane);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      multiply(1);
+      __builtin_amdgcn_sched_barrier(0);
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the next first half, long there
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 };
