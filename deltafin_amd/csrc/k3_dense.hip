@@ -450,6 +450,7 @@ Plan plan_product(int n, int m, int steps, bool glu, Scratch& s) {
   const int64_t slots = p.large ? cus : 2 * cus;
   const int64_t t = tiles(bn, bm);
   int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(t, 1), steps / 8));
+  steps = std::max(steps, 1);
   p.per = (int)((steps + splits - 1) / splits);
   p.splits = (steps + p.per - 1) / p.per;
   p.pitch = (int)round_up((uint32_t)cols, 4);
@@ -489,7 +490,7 @@ int product(GemmArgs a, const Epilogue& e, const Plan& p, const char* what, hipS
   return launched_or(tl, what);
 }
 
-int steps_of(int k) { return (k + kStep - 1) / kStep; }
+int steps_of(int k) { return k / kStep; }  // whole ones
 
 bool vec_ok(int n, int out_elem, std::initializer_list<const void*> ptrs) {
   if (n % 4 != 0) return false;

@@ -33,6 +33,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "k3_device.h"
 
 namespace k3 {
@@ -57,7 +59,7 @@ struct GemmArgs {
   int kw, kx;          // k held by a KMAJOR / INT8 row in memory, whole chunks (>= k)
   uint32_t ldw, ldx;   // bytes between rows
   int tiles_n, tiles_m;
-  int splits, per;     // steps [z * per, ...) of all segments' for grid z
+  int splits, per;     // whole steps [z * per, ...) of all segments' for grid z
 };
 
 __device__ const u32x4 g_zero_chunk = {0u, 0u, 0u, 0u};
@@ -140,27 +142,22 @@ struct Tile {
     }
   }
 
-  // The step at base (the operand's row r0, k = k0; NMAJOR: k = k0, column r0; base2 in the
-  // up matrix) to lds.
-  __device__ __forceinline__ void load(const uint8_t* base, const uint8_t* base2, int wave,
+  // Load i of this wave of the whole step at base (the operand's row r0, k = k0; NMAJOR:
+  // k = k0, column r0; base2 in the up matrix) to lds.
+  __device__ __forceinline__ void load(int i, const uint8_t* base, const uint8_t* base2, int wave,
                                        uint32_t lds) const {
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-      const int j = wave * kPer + i;
-      if (kLoads % WAVES != 0 && j >= kLoads) break;
-      const uint8_t* b = kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base;
-      load_lds(b, off[i], lds + 1024 * j);
-    }
+    const int j = wave * kPer + i;
+    if (kLoads % WAVES != 0 && j >= kLoads) return;
+    load_lds(kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base, off[i], lds + 1024 * j);
   }
 
-  // The same where only `left` < 64 k of the step exist in memory: zeros past them.
+  // The whole share of a step of which `left` < 64 k exist in memory: zeros past them.
   __device__ __forceinline__ void load_tail(const uint8_t* base, const uint8_t* base2, int wave,
                                             int lane, int left, uint32_t lds) const {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int j = wave * kPer + i;
       if (kLoads % WAVES != 0 && j >= kLoads) break;
-      const uint8_t* b = kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base;
       int k;
       if constexpr (L == L_NMAJOR) {
         k = j * (64 / kRowLoads) + lane / kRowLoads;
@@ -170,6 +167,7 @@ struct Tile {
         const int slot = lane % (64 / per);
         k = kChunkK * (L == L_INT8 ? slot ^ int8_swizzle(rl) : slot ^ kmajor_swizzle(rl));
       }
+      const uint8_t* b = kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base;
       load_lds(k < left ? b + off[i] : reinterpret_cast<const uint8_t*>(&g_zero_chunk),
                lds + 1024 * j);
     }
@@ -197,34 +195,38 @@ struct Frags {
   bf16x8 v[2][F];
   u32x4 raw[L == L_INT8 ? F : 1];  // both halves' int8 values as read
 
+  // Where this lane reads block row16 of a tile in half kk.  Opaque, so that it is formed
+  // here each time instead of being held (or, NMAJOR, F of its exclusive-ors being held)
+  // in registers across the loop, which spilled.
   template <int kk>
-  __device__ __forceinline__ void read(const uint8_t* lds, int row16, int lane) {
+  __device__ static __forceinline__ uint32_t place(int row16, int lane) {
     const int i16 = lane & 15, g = lane >> 4;
+    uint32_t at;
     if constexpr (L == L_KMAJOR) {
-      const uint8_t* p = lds + row16 * 2048 + i16 * 128 + (((2 * g + kk) ^ kmajor_swizzle(i16)) << 4);
-#pragma unroll
-      for (int f = 0; f < F; ++f) v[kk][f] = *reinterpret_cast<const bf16x8*>(p + 2048 * f);
+      at = row16 * 2048 + i16 * 128 + (((2 * g + kk) ^ kmajor_swizzle(i16)) << 4);
     } else if constexpr (L == L_INT8) {
-      if constexpr (kk == 0) {
-        const uint8_t* p = lds + row16 * 1024 + i16 * 64 + ((g ^ int8_swizzle(i16)) << 4);
-#pragma unroll
-        for (int f = 0; f < F; ++f) raw[f] = *reinterpret_cast<const u32x4*>(p + 1024 * f);
-      }
+      at = row16 * 1024 + i16 * 64 + ((g ^ int8_swizzle(i16)) << 4);
     } else {
       const int kr = 16 * g + 8 * kk + (i16 >> 2);  // and kr + 4: the same swizzle
-      // the chunk's place; opaque, so that the F exclusive-ors stay here instead of in F
-      // registers across the loop (which spilled)
-      uint32_t at = kr * (2 * R) + (i16 & 3) * 8 + ((row16 ^ nmajor_swizzle<R>(kr)) << 5);
-      asm volatile("" : "+v"(at));
-#pragma unroll
-      for (int f = 0; f < F; ++f) {
-        const uint8_t* q = lds + (at ^ (f << 5));
-        typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
-        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 8 * R));
-        const bf16x4 a = __builtin_bit_cast(bf16x4, lo), b = __builtin_bit_cast(bf16x4, hi);
-        v[kk][f] = bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-      }
+      at = kr * (2 * R) + (i16 & 3) * 8 + ((row16 ^ nmajor_swizzle<R>(kr)) << 5);
+    }
+    return at;
+  }
+
+  // Block f of half kk, `at` being place<kk>.  int8 blocks come whole with the first half.
+  template <int kk>
+  __device__ __forceinline__ void read(int f, const uint8_t* tile, uint32_t at) {
+    if constexpr (L == L_KMAJOR) {
+      v[kk][f] = *reinterpret_cast<const bf16x8*>(tile + at + 2048 * f);
+    } else if constexpr (L == L_INT8) {
+      if constexpr (kk == 0) raw[f] = *reinterpret_cast<const u32x4*>(tile + at + 1024 * f);
+    } else {
+      typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
+      const uint8_t* q = tile + (at ^ (f << 5));
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
+      const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 8 * R));
+      const bf16x4 a = __builtin_bit_cast(bf16x4, lo), b = __builtin_bit_cast(bf16x4, hi);
+      v[kk][f] = bf16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     }
   }
 
@@ -275,8 +277,10 @@ struct Core {
     tx.init(wave, lane, rm, a.m, a.ldx);
     const uint64_t w0 = WL == L_NMAJOR ? (uint64_t)rn * 2 : (uint64_t)rn * a.ldw;
     const uint64_t x0 = XL == L_NMAJOR ? (uint64_t)rm * 2 : (uint64_t)rm * a.ldx;
-    const int steps = (a.k + kStep - 1) / kStep;
-    const int s0 = split * a.per, s1 = min(s0 + a.per, steps * a.segments);
+    // whole steps of every segment, then each segment's rest in the last split
+    const int steps = a.k / kStep;
+    const int s0 = min(split * a.per, steps * a.segments);
+    const int s1 = min(s0 + a.per, steps * a.segments);
 
 #pragma unroll
     for (int i = 0; i < FN; ++i)
@@ -284,75 +288,135 @@ struct Core {
       for (int j = 0; j < FM; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
     // where the next step comes from: pointers that advance, read anew per segment
-    int seg = s0 / steps, k0 = (s0 - seg * steps) * kStep;
     const uint64_t dw = WL == L_NMAJOR ? (uint64_t)kStep * a.ldw : kStep * (WL == L_INT8 ? 1 : 2);
     const uint64_t dx = XL == L_NMAJOR ? (uint64_t)kStep * a.ldx : kStep * 2;
+    int seg = 0, left = 0;  // steps of the segment from the next one on
     const uint8_t *pw = nullptr, *pu = nullptr, *px = nullptr;
     auto open = [&](int step) {
       pw = a.w[seg] + w0 + step * dw;
       if constexpr (kPairs) pu = a.w2[seg] + w0 + step * dw;
       px = a.x[seg] + x0 + step * dx;
+      left = steps - step;
     };
-    auto load = [&](uint32_t buf) {
-      if (__builtin_expect(k0 + kStep > a.kw, 0))
-        tw.load_tail(pw, pu, wave, lane, a.kw - k0, buf);
+    auto load = [&](int i, uint32_t buf) {  // load i of the step's kLoads of this wave
+      if (i < TW::kPer)
+        tw.load(i, pw, pu, wave, buf);
       else
-        tw.load(pw, pu, wave, buf);
-      if (__builtin_expect(k0 + kStep > a.kx, 0))
-        tx.load_tail(px, nullptr, wave, lane, a.kx - k0, buf + TW::kBytes);
-      else
-        tx.load(px, nullptr, wave, buf + TW::kBytes);
-      k0 += kStep;
+        tx.load(i - TW::kPer, px, nullptr, wave, buf + TW::kBytes);
+    };
+    constexpr int kLoads = TW::kPer + TX::kPer;
+    auto advance = [&] {
       pw += dw;
       if constexpr (kPairs) pu += dw;
       px += dx;
-      if (k0 >= a.k && ++seg < a.segments) {
-        k0 = 0;
-        open(0);
-      }
+      if (--left == 0 && ++seg < a.segments) open(0);
     };
-    if (s0 >= s1) return;
-    Frags<BN, WL, FN> fw;
-    Frags<BM, XL, FM> fx;
-    auto multiply = [&](int kk) {
+    typedef Frags<BN, WL, FN> FW;
+    typedef Frags<BM, XL, FM> FX;
+    FW fw;
+    FX fx;
+    // block b of the FN + FM that a half step needs
+    auto read = [&](auto half, int b, const uint8_t* tile, uint32_t at_w, uint32_t at_x) {
+      constexpr int kk = decltype(half)::value;
+      if (b < FN)
+        fw.template read<kk>(b, tile, at_w);
+      else
+        fx.template read<kk>(b - FN, tile + TW::kBytes, at_x);
+    };
+    // Half kk's products, a column of FN at a time; between the columns go the reads of
+    // the other half (from `tile`, if any) and the loads of a later step (if any), few at a
+    // time: 64 loads of 1 KB issued together keep the waves from their products for the
+    // 1000 cycles that the address units take over them.
+    constexpr int kReads = (FN + FM + FM - 2) / (FM - 1);  // per column, none behind the last
+    constexpr int kLoadsPer = (kLoads + FM - 1) / FM;
+    auto half = [&](auto kk_, auto reads_, auto loads_, const uint8_t* tile, uint32_t buf) {
+      constexpr int kk = decltype(kk_)::value;
+      constexpr bool reads = decltype(reads_)::value, loads = decltype(loads_)::value;
+      std::integral_constant<int, 1 - kk> other;
+      const uint32_t at_w = FW::template place<1 - kk>(wn * FN, lane);
+      const uint32_t at_x = FX::template place<1 - kk>(wm * FM, lane);
+      fw.template widen<kk>();
 #pragma unroll
-      for (int j = 0; j < FM; ++j)
+      for (int j = 0; j < FM; ++j) {
 #pragma unroll
         for (int i = 0; i < FN; ++i)
           acc[i][j] =
               __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw.v[kk][i], fx.v[kk][j], acc[i][j], 0, 0, 0);
-    };
-    open(k0 / kStep);
-    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    load(lds0);
-    landed();
-    if (s0 + 1 < s1) load(lds0 + kBuffer);
-    fw.template read<0>(lds, wn * FN, lane);
-    fx.template read<0>(lds + TW::kBytes, wm * FM, lane);
-    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0)
-    for (int s = s0; s < s1; ++s) {
-      uint8_t* cur = lds + ((s - s0) & 1) * kBuffer;
-      uint8_t* nxt = lds + ((s - s0 + 1) & 1) * kBuffer;
-      // the first half's products cover the reads of the second
-      fw.template read<1>(cur, wn * FN, lane);
-      fx.template read<1>(cur + TW::kBytes, wm * FM, lane);
-      __builtin_amdgcn_sched_barrier(0);
-      fw.template widen<0>();
-      multiply(0);
-      fw.template widen<1>();
-      __builtin_amdgcn_sched_barrier(0);
-      // the next step has landed and nobody reads this one any more
-      landed();
-      if (s + 2 < s1) load(lds0 + ((s - s0) & 1) * kBuffer);
-      if (s + 1 < s1) {
-        fw.template read<0>(nxt, wn * FN, lane);
-        fx.template read<0>(nxt + TW::kBytes, wm * FM, lane);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (loads) {
+#pragma unroll
+          for (int i = j * kLoadsPer; i < (j + 1) * kLoadsPer; ++i)
+            if (i < kLoads) load(i, buf);
+        }
+        if constexpr (reads) {
+#pragma unroll
+          for (int b = j * kReads; b < (j + 1) * kReads; ++b)
+            if (b < FN + FM) read(other, b, tile, at_w, at_x);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
+      if constexpr (loads) advance();
+    };
+    const std::integral_constant<int, 0> h0;
+    const std::integral_constant<int, 1> h1;
+    const std::true_type yes;
+    const std::false_type no;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    auto first_half = [&](const uint8_t* tile) {
+      const uint32_t at_w = FW::template place<0>(wn * FN, lane);
+      const uint32_t at_x = FX::template place<0>(wm * FM, lane);
+#pragma unroll
+      for (int b = 0; b < FN + FM; ++b) read(h0, b, tile, at_w, at_x);
+    };
+    auto blocks_there = [] {
+      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): issued a half step ago
       __builtin_amdgcn_sched_barrier(0);
-      multiply(1);
-      __builtin_amdgcn_sched_barrier(0);
-      __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the next first half, long there
-      __builtin_amdgcn_sched_barrier(0);
+    };
+    if (s0 < s1) {
+      auto load_all = [&](uint32_t buf) {
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) load(i, buf);
+        advance();
+      };
+      seg = s0 / steps;
+      open(s0 - seg * steps);
+      load_all(lds0);
+      landed();
+      if (s0 + 1 < s1) load_all(lds0 + kBuffer);
+      first_half(lds);
+      uint32_t at = 0;  // buffer of the step
+      for (int s = s0; s < s1 - 2; ++s) {
+        blocks_there();
+        half(h0, yes, no, lds + at, 0);
+        landed();  // the next step is there and nobody reads this one any more
+        __builtin_amdgcn_sched_barrier(0);
+        half(h1, yes, yes, lds + (kBuffer - at), lds0 + at);
+        at = kBuffer - at;
+      }
+      if (s0 + 1 < s1) {
+        blocks_there();
+        half(h0, yes, no, lds + at, 0);
+        landed();
+        __builtin_amdgcn_sched_barrier(0);
+        half(h1, yes, no, lds + (kBuffer - at), 0);
+        at = kBuffer - at;
+      }
+      blocks_there();
+      half(h0, yes, no, lds + at, 0);
+      half(h1, no, no, lds, 0);
+    }
+    const int rest = a.k - steps * kStep;
+    if (rest > 0 && split == a.splits - 1) {
+      for (seg = 0; seg < a.segments; ++seg) {
+        open(steps);
+        __syncthreads();  // the buffer is no longer read
+        tw.load_tail(pw, pu, wave, lane, a.kw - steps * kStep, lds0);
+        tx.load_tail(px, nullptr, wave, lane, a.kx - steps * kStep, lds0 + TW::kBytes);
+        landed();
+        first_half(lds);
+        half(h0, yes, no, lds, 0);
+        half(h1, no, no, lds, 0);
+      }
     }
   }
 };
