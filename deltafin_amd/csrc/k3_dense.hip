@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * NWN * NWM) void k_gemm(const GemmArgs a, const
                                                          float* part, int pitch) {
   constexpr bool kGlu = EPI == EPI_GLU;
   typedef Core<BN, BM, NWN, NWM, WL, XL, kGlu> C;
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * C::kBuffer];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[C::kLds];
   int tn, tm;
   tile_of(blockIdx.x, a.tiles_n, a.tiles_m, &tn, &tm);
   f32x4 acc[C::FN][C::FM];

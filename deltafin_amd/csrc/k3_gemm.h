@@ -82,9 +82,11 @@ __device__ __forceinline__ void load_lds(const uint8_t* lane_address, uint32_t l
                : "s"(lds), "v"(lane_address)
                : "memory");
 }
-// All of this wave's loads have landed, then everybody's.
+// All but the last N of this wave's loads have landed, then everybody's.
+template <int N>
 __device__ __forceinline__ void landed() {
-  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  static_assert(N < 16, "the counter's low bits");
+  __builtin_amdgcn_s_waitcnt(0x0f70 | N);
   __syncthreads();
 }
 
@@ -111,7 +113,7 @@ template <int R, int L, int WAVES, bool kPairs>
 struct Tile {
   static constexpr int kBytes = R * kStep * (L == L_INT8 ? 1 : 2);
   static constexpr int kLoads = kBytes / 1024;                      // wave instructions
-  static constexpr int kPer = (kLoads + WAVES - 1) / WAVES;         // of one wave
+  static constexpr int kPer = kLoads / WAVES;                       // of one wave
   static constexpr int kChunkK = L == L_INT8 ? 16 : 8;              // k of a 16-byte chunk
   static constexpr int kRowLoads = R / 8;                           // NMAJOR: chunks of a k row
   static_assert(kLoads * 1024 == kBytes, "whole instructions");
@@ -147,7 +149,6 @@ struct Tile {
   __device__ __forceinline__ void load(int i, const uint8_t* base, const uint8_t* base2, int wave,
                                        uint32_t lds) const {
     const int j = wave * kPer + i;
-    if (kLoads % WAVES != 0 && j >= kLoads) return;
     load_lds(kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base, off[i], lds + 1024 * j);
   }
 
@@ -157,7 +158,6 @@ struct Tile {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       const int j = wave * kPer + i;
-      if (kLoads % WAVES != 0 && j >= kLoads) break;
       int k;
       if constexpr (L == L_NMAJOR) {
         k = j * (64 / kRowLoads) + lane / kRowLoads;
@@ -263,7 +263,12 @@ struct Core {
   static constexpr int FN = BN / 16 / NWN, FM = BM / 16 / NWM;
   typedef Tile<BN, WL, kWaves, kPairs> TW;
   typedef Tile<BM, XL, kWaves, false> TX;
-  static constexpr int kBuffer = TW::kBytes + TX::kBytes;
+  static_assert(TW::kLoads % kWaves == 0 && TX::kLoads % kWaves == 0, "equal shares of loads");
+  // Three tiles of the weight side and two of the other: 160 KB, all of a CU's LDS, at 256 x
+  // 256 BF16.  Half of a step's loads are issued two steps ahead, the others, the first
+  // after the barrier that frees their tile, one.
+  static constexpr int kSlotX = 3 * TW::kBytes;  // offset of the second operand's tiles
+  static constexpr int kLds = kSlotX + 2 * TX::kBytes;
 
   __device__ static __forceinline__ void run(const GemmArgs& a, uint8_t* lds, int tn, int tm,
                                              int split, f32x4 (&acc)[FN][FM]) {
@@ -290,48 +295,49 @@ struct Core {
     // where the next step comes from: pointers that advance, read anew per segment
     const uint64_t dw = WL == L_NMAJOR ? (uint64_t)kStep * a.ldw : kStep * (WL == L_INT8 ? 1 : 2);
     const uint64_t dx = XL == L_NMAJOR ? (uint64_t)kStep * a.ldx : kStep * 2;
-    int seg = 0, left = 0;  // steps of the segment from the next one on
     const uint8_t *pw = nullptr, *pu = nullptr, *px = nullptr;
-    auto open = [&](int step) {
-      pw = a.w[seg] + w0 + step * dw;
-      if constexpr (kPairs) pu = a.w2[seg] + w0 + step * dw;
-      px = a.x[seg] + x0 + step * dx;
-      left = steps - step;
+    int segw = 0, leftw = 0, segx = 0, leftx = 0;  // steps of the segment from the next one on
+    auto open_w = [&](int step) {
+      pw = a.w[segw] + w0 + step * dw;
+      if constexpr (kPairs) pu = a.w2[segw] + w0 + step * dw;
+      leftw = steps - step;
     };
-    auto load = [&](int i, uint32_t buf) {  // load i of the step's kLoads of this wave
-      if (i < TW::kPer)
-        tw.load(i, pw, pu, wave, buf);
-      else
-        tx.load(i - TW::kPer, px, nullptr, wave, buf + TW::kBytes);
+    auto open_x = [&](int step) {
+      px = a.x[segx] + x0 + step * dx;
+      leftx = steps - step;
     };
-    constexpr int kLoads = TW::kPer + TX::kPer;
-    auto advance = [&] {
+    auto advance_w = [&] {
       pw += dw;
       if constexpr (kPairs) pu += dw;
+      if (--leftw == 0 && ++segw < a.segments) open_w(0);
+    };
+    auto advance_x = [&] {
       px += dx;
-      if (--left == 0 && ++seg < a.segments) open(0);
+      if (--leftx == 0 && ++segx < a.segments) open_x(0);
     };
     typedef Frags<BN, WL, FN> FW;
     typedef Frags<BM, XL, FM> FX;
     FW fw;
     FX fx;
     // block b of the FN + FM that a half step needs
-    auto read = [&](auto half, int b, const uint8_t* tile, uint32_t at_w, uint32_t at_x) {
+    auto read = [&](auto half, int b, const uint8_t* tw_at, const uint8_t* tx_at, uint32_t at_w,
+                    uint32_t at_x) {
       constexpr int kk = decltype(half)::value;
       if (b < FN)
-        fw.template read<kk>(b, tile, at_w);
+        fw.template read<kk>(b, tw_at, at_w);
       else
-        fx.template read<kk>(b - FN, tile + TW::kBytes, at_x);
+        fx.template read<kk>(b - FN, tx_at, at_x);
     };
-    // Half kk's products, a column of FN at a time; between the columns go the reads of
-    // the other half (from `tile`, if any) and the loads of a later step (if any), few at a
-    // time: 64 loads of 1 KB issued together keep the waves from their products for the
-    // 1000 cycles that the address units take over them.
+    // Half kk's products, a column of FN at a time; between the columns go the loads of
+    // later steps, then the reads of the other half, few at a time: 64 loads of 1 KB issued
+    // together keep the waves from their products for the 1000 cycles that the address
+    // units take over them.
     constexpr int kReads = (FN + FM + FM - 2) / (FM - 1);  // per column, none behind the last
-    constexpr int kLoadsPer = (kLoads + FM - 1) / FM;
-    auto half = [&](auto kk_, auto reads_, auto loads_, const uint8_t* tile, uint32_t buf) {
+    constexpr int kLoadsPer = (TW::kPer + TX::kPer + FM - 1) / FM;
+    auto half = [&](auto kk_, auto reads_, auto load_x, auto load_w, const uint8_t* tw_at,
+                    const uint8_t* tx_at, uint32_t to_x, uint32_t to_w) {
       constexpr int kk = decltype(kk_)::value;
-      constexpr bool reads = decltype(reads_)::value, loads = decltype(loads_)::value;
+      constexpr bool lx = decltype(load_x)::value, lw = decltype(load_w)::value;
       std::integral_constant<int, 1 - kk> other;
       const uint32_t at_w = FW::template place<1 - kk>(wn * FN, lane);
       const uint32_t at_x = FX::template place<1 - kk>(wm * FM, lane);
@@ -343,79 +349,95 @@ struct Core {
           acc[i][j] =
               __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw.v[kk][i], fx.v[kk][j], acc[i][j], 0, 0, 0);
         __builtin_amdgcn_sched_barrier(0);
-        if constexpr (loads) {
 #pragma unroll
-          for (int i = j * kLoadsPer; i < (j + 1) * kLoadsPer; ++i)
-            if (i < kLoads) load(i, buf);
+        for (int i = j * kLoadsPer; i < (j + 1) * kLoadsPer; ++i) {
+          if (lx && i < TX::kPer) tx.load(i, px, nullptr, wave, to_x);
+          if (lw && i >= TX::kPer && i < TX::kPer + TW::kPer)
+            tw.load(i - TX::kPer, pw, pu, wave, to_w);
         }
-        if constexpr (reads) {
+        if constexpr (decltype(reads_)::value) {
 #pragma unroll
           for (int b = j * kReads; b < (j + 1) * kReads; ++b)
-            if (b < FN + FM) read(other, b, tile, at_w, at_x);
+            if (b < FN + FM) read(other, b, tw_at, tx_at, at_w, at_x);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
-      if constexpr (loads) advance();
+      if constexpr (lx) advance_x();
+      if constexpr (lw) advance_w();
     };
     const std::integral_constant<int, 0> h0;
     const std::integral_constant<int, 1> h1;
     const std::true_type yes;
     const std::false_type no;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    auto first_half = [&](const uint8_t* tile) {
+    auto first_half = [&] {  // of the step in the first slots
       const uint32_t at_w = FW::template place<0>(wn * FN, lane);
       const uint32_t at_x = FX::template place<0>(wm * FM, lane);
 #pragma unroll
-      for (int b = 0; b < FN + FM; ++b) read(h0, b, tile, at_w, at_x);
+      for (int b = 0; b < FN + FM; ++b) read(h0, b, lds, lds + kSlotX, at_w, at_x);
     };
     auto blocks_there = [] {
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): issued a half step ago
       __builtin_amdgcn_sched_barrier(0);
     };
     if (s0 < s1) {
-      auto load_all = [&](uint32_t buf) {
+      auto all_w = [&](uint32_t to) {
 #pragma unroll
-        for (int i = 0; i < kLoads; ++i) load(i, buf);
-        advance();
+        for (int i = 0; i < TW::kPer; ++i) tw.load(i, pw, pu, wave, to);
+        advance_w();
       };
-      seg = s0 / steps;
-      open(s0 - seg * steps);
-      load_all(lds0);
-      landed();
-      if (s0 + 1 < s1) load_all(lds0 + kBuffer);
-      first_half(lds);
-      uint32_t at = 0;  // buffer of the step
-      for (int s = s0; s < s1 - 2; ++s) {
-        blocks_there();
-        half(h0, yes, no, lds + at, 0);
-        landed();  // the next step is there and nobody reads this one any more
-        __builtin_amdgcn_sched_barrier(0);
-        half(h1, yes, yes, lds + (kBuffer - at), lds0 + at);
-        at = kBuffer - at;
+      auto all_x = [&](uint32_t to) {
+#pragma unroll
+        for (int i = 0; i < TX::kPer; ++i) tx.load(i, px, nullptr, wave, to);
+        advance_x();
+      };
+      const int n = s1 - s0;
+      segw = segx = s0 / steps;
+      open_w(s0 - segw * steps);
+      open_x(s0 - segx * steps);
+      all_w(lds0);
+      all_x(lds0 + kSlotX);
+      landed<0>();
+      if (n > 1) {
+        all_w(lds0 + TW::kBytes);
+        all_x(lds0 + kSlotX + TX::kBytes);
       }
-      if (s0 + 1 < s1) {
+      if (n > 2) all_w(lds0 + 2 * TW::kBytes);
+      first_half();
+      uint32_t w_at = 0, x_at = kSlotX;  // the step's tiles
+      auto next_w = [&] { return w_at == 2 * TW::kBytes ? 0u : w_at + (uint32_t)TW::kBytes; };
+      auto next_x = [&] { return 2 * kSlotX + TX::kBytes - x_at; };
+      // A step: its first half, the barrier behind which the next step's tiles are there and
+      // its own are free, its second half.
+      auto step = [&](auto wait, auto reads, auto load_x, auto load_w) {
         blocks_there();
-        half(h0, yes, no, lds + at, 0);
-        landed();
-        __builtin_amdgcn_sched_barrier(0);
-        half(h1, yes, no, lds + (kBuffer - at), 0);
-        at = kBuffer - at;
-      }
-      blocks_there();
-      half(h0, yes, no, lds + at, 0);
-      half(h1, no, no, lds, 0);
+        half(h0, yes, no, no, lds + w_at, lds + x_at, 0, 0);
+        if constexpr (decltype(reads)::value) {
+          landed<decltype(wait)::value>();
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        half(h1, reads, load_x, load_w, lds + next_w(), lds + next_x(), lds0 + x_at, lds0 + w_at);
+        w_at = next_w();
+        x_at = next_x();
+      };
+      const std::integral_constant<int, TW::kPer> ahead;  // loads of the tile two steps on
+      for (int s = 0; s < n - 3; ++s) step(ahead, yes, yes, yes);
+      if (n > 2) step(ahead, yes, yes, no);
+      if (n > 1) step(h0, yes, no, no);
+      step(h0, no, no, no);
     }
     const int rest = a.k - steps * kStep;
     if (rest > 0 && split == a.splits - 1) {
-      for (seg = 0; seg < a.segments; ++seg) {
-        open(steps);
-        __syncthreads();  // the buffer is no longer read
+      for (segw = segx = 0; segw < a.segments; ++segw, ++segx) {
+        open_w(steps);
+        open_x(steps);
+        __syncthreads();  // the first slots are no longer read
         tw.load_tail(pw, pu, wave, lane, a.kw - steps * kStep, lds0);
-        tx.load_tail(px, nullptr, wave, lane, a.kx - steps * kStep, lds0 + TW::kBytes);
-        landed();
-        first_half(lds);
-        half(h0, yes, no, lds, 0);
-        half(h1, no, no, lds, 0);
+        tx.load_tail(px, nullptr, wave, lane, a.kx - steps * kStep, lds0 + kSlotX);
+        landed<0>();
+        first_half();
+        half(h0, yes, no, no, lds, lds + kSlotX, 0, 0);
+        half(h1, no, no, no, lds, lds, 0, 0);
       }
     }
   }
