@@ -18,6 +18,7 @@
 #include "k3_gemm.h"
 #include "k3_internal.h"
 #include "k3_launch.h"
+#include "k3_skinny.h"
 
 namespace k3 {
 namespace {
@@ -86,12 +87,6 @@ __device__ __forceinline__ f32x4 load4(const Epilogue& e, const void* p, int bf1
   return v;
 }
 
-__device__ __forceinline__ float unary(int act, float z) {
-  if (act == K3_DENSE_ACT_SILU) return z / (1.0f + expf(-z));
-  if (act == K3_DENSE_ACT_GELU) return 0.5f * z * erfcf(-0.70710678118654752f * z);
-  return z;
-}
-
 // Sums v (GLU: of gate, u of up) of row m, columns n .. n + 3.
 template <int EPI>
 __device__ __forceinline__ void finish(const Epilogue& e, int m, int n, f32x4 v, f32x4 u) {
@@ -132,7 +127,7 @@ __device__ __forceinline__ void finish(const Epilogue& e, int m, int n, f32x4 v,
     if (e.bias) v += load4(e, e.bias, 0, 0, n);
     if (e.act != K3_DENSE_ACT_NONE) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[i] = unary(e.act, v[i]);
+      for (int i = 0; i < 4; ++i) v[i] = unary_activation(e.act, v[i]);
     }
     if (e.res) v += load4(e, e.res, e.bf16, row, n);
     store4(e, e.out, row, n, v);
@@ -500,6 +495,50 @@ bool vec_ok(int n, int out_elem, std::initializer_list<const void*> ptrs) {
   return true;
 }
 
+// Few positions: the skinny kernels stream a matrix once per 16 positions with no scratch
+// memory and no second launch.
+constexpr int kSkinnyPositions = 16;
+bool skinny_linear(const K3HipLinearV1& op, SkinnyOp* sk) {
+  if (op.positions > kSkinnyPositions) return false;
+  sk->kind = op.matrix_kind == K3_SPINE_MATRIX_INT8 ? SKINNY_INT8 : SKINNY_BF16;
+  sk->w = op.weights;
+  sk->row_scales = op.row_scales;
+  sk->x = op.x;
+  sk->x_dtype = (int)op.x_dtype;
+  sk->y = op.out;
+  sk->bias = op.bias;
+  sk->unary = (int)op.activation;
+  sk->add = op.residual;
+  sk->add_bf16 = sk->out_bf16 = op.out_dtype == K3_DTYPE_BF16;
+  sk->rows = (int)op.rows;
+  sk->cols = (int)op.columns;
+  sk->positions = (int)op.positions;
+  return skinny_fits(*sk);
+}
+bool skinny_gated(const K3HipGatedV1& op, SkinnyOp* sk) {
+  if (op.positions > kSkinnyPositions) return false;
+  sk->kind = op.matrix_kind == K3_SPINE_MATRIX_INT8 ? SKINNY_INT8 : SKINNY_BF16;
+  sk->w = op.gate;
+  sk->w2 = op.up;
+  sk->row_scales = op.gate_scales;
+  sk->row_scales2 = op.up_scales;
+  sk->act = (int)op.activation;
+  sk->x = op.x;
+  sk->x_dtype = (int)op.x_dtype;
+  sk->y = op.out;
+  sk->keep_gate = op.out_gate;
+  sk->keep_up = op.out_up;
+  sk->out_bf16 = op.out_dtype == K3_DTYPE_BF16;
+  sk->rows = (int)op.rows;
+  sk->cols = (int)op.columns;
+  sk->positions = (int)op.positions;
+  return skinny_fits(*sk);
+}
+int run_skinny(const SkinnyOp& sk, const char* what, hipStream_t st) {
+  if (launch_skinny(sk, KC_SPINE_MFMA, st) == K3_HIP_OK) return K3_SPINE_OK;
+  return spine_fail(K3_SPINE_E_RUNTIME, "%s: %s", what, k3_hip_last_error());
+}
+
 struct LinearCall {
   Scratch s;
   Matrix w;
@@ -555,9 +594,13 @@ struct GradCall {
 }  // namespace
 
 uint64_t dense_linear_workspace(const K3HipLinearV1& op) {
+  SkinnyOp sk{};
+  if (skinny_linear(op, &sk)) return 256;
   return std::max<uint64_t>(256, LinearCall(op, nullptr).s.used);
 }
 uint64_t dense_gated_workspace(const K3HipGatedV1& op) {
+  SkinnyOp sk{};
+  if (skinny_gated(op, &sk)) return 256;
   return std::max<uint64_t>(256, GatedCall(op, nullptr).s.used);
 }
 uint64_t dense_gated_grad_workspace(const K3HipGatedGradV1& op) {
@@ -565,6 +608,8 @@ uint64_t dense_gated_grad_workspace(const K3HipGatedGradV1& op) {
 }
 
 int dense_linear(const K3HipLinearV1& op, void* ws, hipStream_t st) {
+  SkinnyOp sk{};
+  if (skinny_linear(op, &sk)) return run_skinny(sk, "linear", st);
   const LinearCall c(op, ws);
   int rc = c.w.fill(st);
   if (rc == K3_SPINE_OK) rc = c.x.fill(st);
@@ -599,6 +644,8 @@ int dense_linear(const K3HipLinearV1& op, void* ws, hipStream_t st) {
 }
 
 int dense_gated(const K3HipGatedV1& op, void* ws, hipStream_t st) {
+  SkinnyOp sk{};
+  if (skinny_gated(op, &sk)) return run_skinny(sk, "gated feed-forward", st);
   const GatedCall c(op, ws);
   int rc = c.g.fill(st);
   if (rc == K3_SPINE_OK) rc = c.u.fill(st);

@@ -260,6 +260,14 @@ __device__ __forceinline__ float activate(int act, float g, float u) {
   return (4.0f * tanhf(g / 4.0f) * sig) * (25.0f * tanhf(u / 25.0f));
 }
 
+// A projection's activation (K3_DENSE_ACT_*).  erfc keeps the small values of far negative
+// z that 1 + erf would round away.
+__device__ __forceinline__ float unary_activation(int act, float z) {
+  if (act == 1) return z / (1.0f + expf(-z));
+  if (act == 2) return 0.5f * z * erfcf(-0.70710678118654752f * z);
+  return z;
+}
+
 // ---------------------------------------------------------------- loads
 // Global-address-space views: loads through them compile to global_load (vmcnt
 // only) rather than flat_load, which would also count against lgkmcnt and make

@@ -19,10 +19,15 @@ struct SkinnyOp {
   const uint8_t* scales2;
   int act;                     // GLU: K3_ACT_*
   const void* x;               // [positions, cols]
-  int x_dtype;                 // K3_DTYPE_*; BF16 only for SKINNY_FP4 without w2
+  int x_dtype;                 // K3_DTYPE_*; with w2, SKINNY_FP4 takes fp32 only
   void* y;                     // [positions, rows]
   float* y_up;                 // GLU: w2 . x when non-null
-  const float* add;            // y += add [positions, rows] (fp32, no GLU; may be y)
+  void* keep_gate;             // GLU: w . x and w2 . x in y's type, both or neither
+  void* keep_up;
+  const float* bias;           // [rows], no GLU
+  int unary;                   // K3_DENSE_ACT_*, no GLU
+  const void* add;             // y += add [positions, rows] (y's type, no GLU; may be y)
+  int add_bf16;                // add's type
   int out_bf16;
   int rows, cols, positions;
 };

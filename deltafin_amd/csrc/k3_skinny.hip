@@ -40,6 +40,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "k3_device.h"
 #include "k3_internal.h"
@@ -69,45 +70,69 @@ struct SkinnyArgs {
   const void* x;
   void* y;
   float* y_up;       // kGlu: receives up . x when non-null
-  const float* add;  // added to an fp32 result when non-null
+  void* keep[2];     // kGlu: receive gate . x and up . x in y's type when non-null
+  const float* bias;
+  const void* add;   // added to a result when non-null, in y's type
   int rows, cols, P;
   int lines;      // 128-byte lines of a row, the last one possibly partial
   int tail;       // bytes of the last line
   int S, per;     // waves splitting the lines, lines of a wave
   int out_bf16, act;
+  int unary;  // K3_DENSE_ACT_* of a single product
 };
 
-// Activation blocks: 256 bytes of each row, operands of one block and blocks
-// of one weight line.
+// BF16 activation rows in blocks of 64 columns, as many as a BF16 weight line has (the
+// 128 columns of a uint16_t block are two such lines).
+struct Bf16Row64 {
+  uint16_t bits;
+};
+
+// Activation blocks: 256 bytes of each row (Bf16Row64: 128), operands of one block and
+// blocks of one weight line.
+template <typename XT>
+constexpr int block_columns() {
+  return std::is_same<XT, Bf16Row64>::value ? 64 : 256 / (int)sizeof(XT);
+}
 template <typename XT>
 constexpr int block_operands() {
-  return 8 / (int)sizeof(XT);
+  return block_columns<XT>() / 32;
 }
 template <int kW, typename XT>
 constexpr int line_blocks() {
   return 2 * operands<kW>() / block_operands<XT>();
 }
+// What a lane loads of a block's row: a sixteenth.
+template <typename XT>
+struct LaneLoad {
+  typedef u32x4 type;
+};
+template <>
+struct LaneLoad<Bf16Row64> {
+  typedef uint32_t type __attribute__((ext_vector_type(2)));
+};
 
-// A block goes to LDS as loaded (BF16 activations; fp32 ones of four row quads
-// or more) or as its three terms: splitting before the store splits every value
+// A block goes to LDS as loaded (128 columns of BF16 activations; fp32 ones of four row
+// quads or more), as its three terms, or as its one (Bf16Row64): splitting before the
+// store splits every value
 // once instead of once per 16 columns of the operand read, which pays while the
 // rows are fewer than those columns; a split row costs 6 bytes of LDS traffic
 // each way instead of 4.
 template <typename XT, int RQ>
 constexpr bool raw_blocks() {
-  return sizeof(XT) == 2 || RQ >= 4;
+  return std::is_same<XT, uint16_t>::value || (sizeof(XT) == 4 && RQ >= 4);
 }
 // 16-byte LDS slots of a block.
 template <typename XT, int RQ>
 constexpr int block_f4() {
-  return RQ * 4 * 16 * (raw_blocks<XT, RQ>() ? 2 : 3) / 2;
+  return RQ * 4 * 8 *
+         (raw_blocks<XT, RQ>() ? 2 : sizeof(XT) == 4 ? 3 : 1);
 }
 
 // One line's worth of loads.
 template <int kW, typename XT, int RQ, int TLT>
 struct Stage {
   u32x4 a[TLT][2];
-  u32x4 x[line_blocks<kW, XT>()][RQ];
+  typename LaneLoad<XT>::type x[line_blocks<kW, XT>()][RQ];
   uint64_t s[kW == SKINNY_FP4 ? TLT : 1];
 };
 
@@ -273,7 +298,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
   constexpr int NT = sizeof(XT) == 4 ? 3 : 1;   // terms of an activation
   constexpr int OB = block_operands<XT>();
   constexpr int NBK = line_blocks<kW, XT>();
-  constexpr int XC = 256 / (int)sizeof(XT);     // columns of a block
+  constexpr int XC = block_columns<XT>();       // columns of a block
   constexpr int kRegions = NBK > 1 ? 2 : 1;
   constexpr bool kRaw = raw_blocks<XT, RQ>();
   constexpr int kTermF4 = RQ * 4 * XC / 8;      // 16-byte slots of a block's term
@@ -329,10 +354,12 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
   auto load_x = [&](St& s, int j) {
 #pragma unroll
     for (int b = 0; b < NBK; ++b) {
-      const uint32_t k = (uint32_t)(j * NBK + b) * XC + (16 / sizeof(XT)) * i16;
+      const uint32_t k = (uint32_t)(j * NBK + b) * XC + (XC / 16) * i16;
       const uint32_t ko = j == tail_line && k >= (uint32_t)args.cols ? 0u : k * sizeof(XT);
 #pragma unroll
-      for (int n = 0; n < RQ; ++n) s.x[b][n] = *(gu32x4*)(xb + (xoff[n] + ko));
+      for (int n = 0; n < RQ; ++n)
+        s.x[b][n] = *(__attribute__((address_space(1))) const typename LaneLoad<XT>::type*)(
+            xb + (xoff[n] + ko));
     }
   };
   auto load_a = [&](St& s, int j) {
@@ -364,6 +391,9 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
     for (int n = 0; n < RQ; ++n) {
       if constexpr (kRaw) {
         r[slot(4 * n + g, i16)] = __builtin_bit_cast(f32x4, s.x[b][n]);
+      } else if constexpr (NT == 1) {
+        reinterpret_cast<uint2*>(r + slot(4 * n + g, i16 >> 1))[i16 & 1] =
+            __builtin_bit_cast(uint2, s.x[b][n]);
       } else {
         uint2 t[3];
         split4(s.x[b][n], t);
@@ -534,16 +564,28 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
     if (!stored) continue;
     const uint64_t yi = (uint64_t)(p0 + p) * rows + row;
     float out = v[0];
+    auto store = [&](void* to, float f) {
+      if (args.out_bf16)
+        static_cast<uint16_t*>(to)[yi] = f32_to_bf16_bits(f);
+      else
+        static_cast<float*>(to)[yi] = f;
+    };
     if constexpr (kGlu) {
       if (args.y_up) args.y_up[yi] = v[1];
+      if (args.keep[0]) {
+        store(args.keep[0], v[0]);
+        store(args.keep[1], v[1]);
+      }
       out = activate(args.act, v[0], v[1]);
-    }
-    if (args.out_bf16) {
-      static_cast<uint16_t*>(args.y)[yi] = f32_to_bf16_bits(out);
     } else {
-      if (!kGlu && args.add) out = args.add[yi] + out;
-      static_cast<float*>(args.y)[yi] = out;
+      if (args.bias) out += args.bias[row];
+      if (args.unary) out = unary_activation(args.unary, out);
+      if (args.add)
+        out = (args.out_bf16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(args.add)[yi])
+                             : static_cast<const float*>(args.add)[yi]) +
+              out;
     }
+    store(args.y, out);
   }
 }
 
@@ -596,18 +638,27 @@ bool go_rows(int TL, const SkinnyArgs& a, hipStream_t st, TimedLaunch& tl) {
 
 // Tiles of gate and as many of up: two of each where one would leave more
 // workgroups than CUs (MXFP4, with its longer lines, always one).
-template <int kW, int RQ>
+template <int kW, typename XT, int RQ>
 bool go_glu_tiles(int TL, const SkinnyArgs& a, hipStream_t st, TimedLaunch& tl) {
   if constexpr (kW != SKINNY_FP4)
-    if (TL > 1) return go<kW, float, RQ, 2, true, 2>(a, st, tl);
-  return go<kW, float, RQ, 1, true, depth<kW, 2>()>(a, st, tl);
+    if (TL > 1) return go<kW, XT, RQ, 2, true, 2>(a, st, tl);
+  return go<kW, XT, RQ, 1, true, depth<kW, 2>()>(a, st, tl);
 }
 
-template <int kW>
+template <int kW, typename XT>
 bool go_glu(int TL, const SkinnyArgs& a, hipStream_t st, TimedLaunch& tl) {
-  if (a.P <= 4) return go_glu_tiles<kW, 1>(TL, a, st, tl);
-  if (a.P <= 8) return go_glu_tiles<kW, 2>(TL, a, st, tl);
-  return go_glu_tiles<kW, 4>(TL, a, st, tl);
+  if (a.P <= 4) return go_glu_tiles<kW, XT, 1>(TL, a, st, tl);
+  if (a.P <= 8) return go_glu_tiles<kW, XT, 2>(TL, a, st, tl);
+  return go_glu_tiles<kW, XT, 4>(TL, a, st, tl);
+}
+
+// BF16 or int8 weights by the activations' type.
+template <int kW>
+bool go_typed(bool glu, bool x_bf16, int TL, const SkinnyArgs& a, hipStream_t st,
+              TimedLaunch& tl) {
+  if (x_bf16)
+    return glu ? go_glu<kW, Bf16Row64>(TL, a, st, tl) : go_rows<kW, Bf16Row64>(TL, a, st, tl);
+  return glu ? go_glu<kW, float>(TL, a, st, tl) : go_rows<kW, float>(TL, a, st, tl);
 }
 
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
@@ -623,8 +674,9 @@ bool skinny_fits(const SkinnyOp& op) {
          row_bytes >= (op.kind == SKINNY_FP4 ? 128u : 64u) && op.cols <= 65536 &&
          op.positions <= (1 << 19) && (uint64_t)op.positions * op.cols <= (1u << 28) &&
          (uint64_t)op.positions * op.rows <= INT32_MAX && aligned16(op.w) && aligned16(op.x) &&
-         (!op.w2 || (aligned16(op.w2) && op.x_dtype == K3_DTYPE_F32)) &&
-         !(op.add && (op.w2 || op.out_bf16));
+         (!op.w2 || (aligned16(op.w2) && (op.x_dtype == K3_DTYPE_F32 || op.kind != SKINNY_FP4))) &&
+         !((op.add || op.bias || op.unary) && op.w2) &&
+         !(op.add && (op.out_bf16 != 0) != (op.add_bf16 != 0));
 }
 
 int launch_skinny(const SkinnyOp& op, int kernel_class, hipStream_t st) {
@@ -635,6 +687,10 @@ int launch_skinny(const SkinnyOp& op, int kernel_class, hipStream_t st) {
   a.sc[1] = op.scales2;
   a.rs[0] = op.row_scales;
   a.rs[1] = op.row_scales2;
+  a.keep[0] = op.keep_gate;
+  a.keep[1] = op.keep_up;
+  a.bias = op.bias;
+  a.unary = op.unary;
   a.add = op.add;
   a.x = op.x;
   a.y = op.y;
@@ -666,12 +722,13 @@ int launch_skinny(const SkinnyOp& op, int kernel_class, hipStream_t st) {
   TimedLaunch tl(kernel_class, st);
   bool ok;
   const bool glu = op.w2 != nullptr;
+  const bool x_bf16 = op.x_dtype == K3_DTYPE_BF16;
   if (op.kind == SKINNY_BF16)
-    ok = glu ? go_glu<SKINNY_BF16>(TL, a, st, tl) : go_rows<SKINNY_BF16, float>(TL, a, st, tl);
+    ok = go_typed<SKINNY_BF16>(glu, x_bf16, TL, a, st, tl);
   else if (op.kind == SKINNY_INT8)
-    ok = glu ? go_glu<SKINNY_INT8>(TL, a, st, tl) : go_rows<SKINNY_INT8, float>(TL, a, st, tl);
-  else if (op.x_dtype == K3_DTYPE_F32)
-    ok = glu ? go_glu<SKINNY_FP4>(TL, a, st, tl) : go_rows<SKINNY_FP4, float>(TL, a, st, tl);
+    ok = go_typed<SKINNY_INT8>(glu, x_bf16, TL, a, st, tl);
+  else if (!x_bf16)
+    ok = glu ? go_glu<SKINNY_FP4, float>(TL, a, st, tl) : go_rows<SKINNY_FP4, float>(TL, a, st, tl);
   else
     ok = go_rows<SKINNY_FP4, uint16_t>(TL, a, st, tl);
   if (!ok) {
