@@ -190,6 +190,7 @@ K3_SAMPLE_MAX_ROWS = 32768
 K3_SAMPLE_MAX_VOCABULARY = 16777216
 K3_DENSE_ABI_V1 = 1
 K3_DENSE_MAX_EXTENT = 1048576
+K3_DENSE_NO_WORKSPACE = 256  # the size of a call that uses no scratch memory
 K3_DENSE_ACT_NONE, K3_DENSE_ACT_SILU, K3_DENSE_ACT_GELU = 0, 1, 2
 
 K3_SPINE_MATRIX_BF16 = 0

@@ -13,7 +13,9 @@
 
 #include <algorithm>
 #include <atomic>
+#include <map>
 #include <mutex>
+#include <tuple>
 #include <string>
 #include <unordered_map>
 #include <vector>
@@ -328,11 +330,10 @@ int device_cu_count() {
 
 bool lds_fits(const void* kernel, int block, size_t dynamic_lds) {
   static std::mutex mu;
-  static std::unordered_map<std::string, bool> cache;
+  static std::map<std::tuple<const void*, int, size_t, int>, bool> cache;
   int dev = 0;
   if (hipGetDevice(&dev) != hipSuccess) dev = -1;
-  char key[96];
-  snprintf(key, sizeof(key), "%p/%d/%zu/%d", kernel, block, dynamic_lds, dev);
+  const auto key = std::make_tuple(kernel, block, dynamic_lds, dev);
   std::lock_guard<std::mutex> lk(mu);
   auto it = cache.find(key);
   if (it != cache.end()) return it->second;

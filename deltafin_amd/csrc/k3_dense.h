@@ -9,7 +9,7 @@
 
 namespace k3 {
 
-// Scratch bytes of a valid descriptor (at least 256).
+// Scratch bytes of a valid descriptor (K3_DENSE_NO_WORKSPACE: none).
 uint64_t dense_linear_workspace(const K3HipLinearV1& op);
 uint64_t dense_gated_workspace(const K3HipGatedV1& op);
 uint64_t dense_gated_grad_workspace(const K3HipGatedGradV1& op);

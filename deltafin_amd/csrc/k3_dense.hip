@@ -595,16 +595,16 @@ struct GradCall {
 
 uint64_t dense_linear_workspace(const K3HipLinearV1& op) {
   SkinnyOp sk{};
-  if (skinny_linear(op, &sk)) return 256;
-  return std::max<uint64_t>(256, LinearCall(op, nullptr).s.used);
+  if (skinny_linear(op, &sk)) return K3_DENSE_NO_WORKSPACE;
+  return K3_DENSE_NO_WORKSPACE + LinearCall(op, nullptr).s.used;
 }
 uint64_t dense_gated_workspace(const K3HipGatedV1& op) {
   SkinnyOp sk{};
-  if (skinny_gated(op, &sk)) return 256;
-  return std::max<uint64_t>(256, GatedCall(op, nullptr).s.used);
+  if (skinny_gated(op, &sk)) return K3_DENSE_NO_WORKSPACE;
+  return K3_DENSE_NO_WORKSPACE + GatedCall(op, nullptr).s.used;
 }
 uint64_t dense_gated_grad_workspace(const K3HipGatedGradV1& op) {
-  return std::max<uint64_t>(256, GradCall(op, nullptr).s.used);
+  return K3_DENSE_NO_WORKSPACE + GradCall(op, nullptr).s.used;
 }
 
 int dense_linear(const K3HipLinearV1& op, void* ws, hipStream_t st) {

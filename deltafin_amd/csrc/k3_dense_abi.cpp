@@ -160,7 +160,8 @@ int check_grad(const K3HipGatedGradV1* op, bool sizes) {
 }
 
 int check_workspace(const char* what, const void* ws, uint64_t bytes, uint64_t need) {
-  if (!ws || ((uintptr_t)ws & 255u) != 0 || bytes < need)
+  const bool none = need == K3_DENSE_NO_WORKSPACE && !ws;
+  if (!none && (!ws || ((uintptr_t)ws & 255u) != 0 || bytes < need))
     return spine_fail(K3_SPINE_E_INVALID,
                       "%s: the workspace must be %llu bytes at a 256-byte boundary, got %llu at %p",
                       what, (unsigned long long)need, (unsigned long long)bytes, ws);
@@ -168,6 +169,16 @@ int check_workspace(const char* what, const void* ws, uint64_t bytes, uint64_t n
   if (e != hipSuccess)
     return spine_fail(K3_SPINE_E_RUNTIME, "%s preflight: %s", what, hipGetErrorString(e));
   return K3_SPINE_OK;
+}
+
+// A call of the C surface: nothing that the host code throws leaves it.
+template <typename F>
+int guarded(const char* what, F f) {
+  try {
+    return f();
+  } catch (...) {
+    return spine_fail(K3_SPINE_E_RUNTIME, "%s: out of host memory", what);
+  }
 }
 
 }  // namespace
@@ -189,7 +200,9 @@ int k3_hip_linear(const K3HipLinearV1* op, void* workspace, uint64_t workspace_b
                   void* stream) {
   K3_TRY(check_linear(op, false));
   K3_TRY(check_workspace("linear", workspace, workspace_bytes, dense_linear_workspace(*op)));
-  return dense_linear(*op, workspace, static_cast<hipStream_t>(stream));
+  return guarded("linear", [&] {
+    return dense_linear(*op, workspace, static_cast<hipStream_t>(stream));
+  });
 }
 
 uint64_t k3_hip_gated_ffn_workspace_bytes(const K3HipGatedV1* op) {
@@ -201,7 +214,9 @@ int k3_hip_gated_ffn(const K3HipGatedV1* op, void* workspace, uint64_t workspace
   K3_TRY(check_gated(op, false));
   K3_TRY(check_workspace("gated feed-forward", workspace, workspace_bytes,
                          dense_gated_workspace(*op)));
-  return dense_gated(*op, workspace, static_cast<hipStream_t>(stream));
+  return guarded("gated feed-forward", [&] {
+    return dense_gated(*op, workspace, static_cast<hipStream_t>(stream));
+  });
 }
 
 uint64_t k3_hip_gated_ffn_grad_workspace_bytes(const K3HipGatedGradV1* op) {
@@ -213,7 +228,9 @@ int k3_hip_gated_ffn_grad(const K3HipGatedGradV1* op, void* workspace, uint64_t 
   K3_TRY(check_grad(op, false));
   K3_TRY(check_workspace("gated feed-forward gradient", workspace, workspace_bytes,
                          dense_gated_grad_workspace(*op)));
-  return dense_gated_grad(*op, workspace, static_cast<hipStream_t>(stream));
+  return guarded("gated feed-forward gradient", [&] {
+    return dense_gated_grad(*op, workspace, static_cast<hipStream_t>(stream));
+  });
 }
 
 }  // extern "C"

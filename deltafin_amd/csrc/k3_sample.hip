@@ -575,8 +575,12 @@ int k3_hip_sample(const K3HipSampleV1* op, void* workspace, uint64_t workspace_b
   while ((1u << bits) < op->vocabulary) ++bits;
   a.shift = 62 - bits;
   hipStream_t st = static_cast<hipStream_t>(stream);
-  return op->logits_dtype == K3_DTYPE_F32 ? sample_launch<float>(a, st)
-                                          : sample_launch<uint16_t>(a, st);
+  try {
+    return op->logits_dtype == K3_DTYPE_F32 ? sample_launch<float>(a, st)
+                                            : sample_launch<uint16_t>(a, st);
+  } catch (...) {
+    return spine_fail(K3_SPINE_E_RUNTIME, "sample: out of host memory");
+  }
 }
 
 }  // extern "C"

@@ -20,41 +20,46 @@ import torch
 from . import _lib
 from .moe import _dtype_code, stream_handle
 
-_BF16_BITS = (torch.int16, torch.uint16, torch.bfloat16)
+_MATRICES = (torch.bfloat16, torch.int8, torch.int16, torch.uint16)
+_ROWS = (torch.float32, torch.bfloat16)
 ACTIVATIONS = {None: _lib.K3_DENSE_ACT_NONE, "none": _lib.K3_DENSE_ACT_NONE,
                "silu": _lib.K3_DENSE_ACT_SILU, "gelu": _lib.K3_DENSE_ACT_GELU}
 GATES = {"situ": _lib.K3_ACT_SITU, "silu": _lib.K3_ACT_SILU}
 
 
 def _check(t: torch.Tensor, dtypes, shape, what: str) -> None:
-    dtypes = dtypes if isinstance(dtypes, tuple) else (dtypes,)
-    if (t.device.type != "cuda" or t.dtype not in dtypes or not t.is_contiguous()
-            or tuple(t.shape) != tuple(shape)):
-        raise ValueError(f"{what} must be a contiguous {' / '.join(map(str, dtypes))} device "
-                         f"tensor of shape {list(shape)}, got {t.dtype} {list(t.shape)} on "
-                         f"{t.device}")
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError(f"{what} is on {t.device}, the current device is "
-                         f"cuda:{torch.cuda.current_device()}")
+    """t is a contiguous tensor of one of the dtypes and the shape on the current device.
+    (One comparison after the other on purpose: a decode step's call is host bound.)"""
+    if (t.dtype is dtypes or t.dtype in dtypes) and t.shape == shape and t.is_contiguous():
+        at = t.get_device()
+        if at >= 0:
+            if at == torch.cuda.current_device():
+                return
+            raise ValueError(f"{what} is on {t.device}, the current device is "
+                             f"cuda:{torch.cuda.current_device()}")
+    names = " / ".join(map(str, dtypes if isinstance(dtypes, tuple) else (dtypes,)))
+    raise ValueError(f"{what} must be a contiguous {names} device tensor of shape "
+                     f"{list(shape)}, got {t.dtype} {list(t.shape)} on {t.device}")
 
 
 def _rows(x: torch.Tensor, columns: int, what: str) -> torch.Tensor:
     """x as [positions, columns]; a single row may come without its first dimension."""
-    if x.dtype not in (torch.float32, torch.bfloat16):
+    if x.dtype not in _ROWS:
         raise ValueError(f"{what} must be float32 or bfloat16, got {x.dtype}")
-    if x.dim() not in (1, 2):
+    if x.dim() == 1:
+        x = x.reshape(1, -1)
+    elif x.dim() != 2:
         raise ValueError(f"{what} must be [columns] or [positions, columns]")
-    x2 = x if x.dim() == 2 else x.view(1, -1) if x.is_contiguous() else x.reshape(1, -1)
-    _check(x2, x.dtype, (x2.shape[0], columns), what)
-    return x2
+    _check(x, x.dtype, (x.shape[0], columns), what)
+    return x
 
 
 def _matrix(w: torch.Tensor, scales: torch.Tensor | None, what: str) -> int:
     """The K3_SPINE_MATRIX_* kind of w, its shape and scales checked."""
     if w.dim() != 2:
         raise ValueError(f"{what} must be 2-D [rows, columns]")
-    _check(w, (*_BF16_BITS, torch.int8), w.shape, what)
-    if w.dtype == torch.int8:
+    _check(w, _MATRICES, w.shape, what)
+    if w.dtype is torch.int8:
         if scales is None:
             raise ValueError(f"int8 {what} needs a scale per row")
         _check(scales, torch.float32, (w.shape[0],), f"{what} scales")
@@ -64,10 +69,16 @@ def _matrix(w: torch.Tensor, scales: torch.Tensor | None, what: str) -> int:
     return _lib.K3_SPINE_MATRIX_BF16
 
 
-def _out(out: torch.Tensor | None, shape, dtype: torch.dtype, what: str) -> torch.Tensor:
+def _out(out: torch.Tensor | None, x: torch.Tensor, rows: int, dtype: torch.dtype | None
+         ) -> torch.Tensor:
+    """The output [positions, rows]: `out`, or a new tensor of the dtype (x's unless given)."""
+    if dtype is None:
+        dtype = x.dtype if out is None else out.dtype
+    if dtype not in _ROWS:
+        raise ValueError(f"outputs are float32 or bfloat16, not {dtype}")
     if out is None:
-        return torch.empty(shape, dtype=dtype, device="cuda")
-    _check(out, dtype, shape, what)
+        return torch.empty((x.shape[0], rows), dtype=dtype, device=x.device)
+    _check(out, dtype, (x.shape[0], rows), "out")
     return out
 
 
@@ -77,15 +88,18 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _run(name: str, d, workspace: torch.Tensor | None) -> None:
     lib = _lib.load()
-    need = getattr(lib, name + "_workspace_bytes")(C.byref(d))
-    if need == 0:
-        raise _lib.K3SpineError(_lib.K3_SPINE_E_INVALID, name + "_workspace_bytes")
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device="cuda")
-    else:
+    ref = C.byref(d)
+    if workspace is not None:
         _check(workspace, torch.uint8, workspace.shape, "workspace")
-    _lib.check_spine(getattr(lib, name)(C.byref(d), workspace.data_ptr(), workspace.numel(),
-                                        stream_handle()), name)
+        at, have = workspace.data_ptr(), workspace.numel()
+    else:
+        at, have = None, getattr(lib, name + "_workspace_bytes")(ref)
+        if have == 0:
+            raise _lib.K3SpineError(_lib.K3_SPINE_E_INVALID, name + "_workspace_bytes")
+        if have > _lib.K3_DENSE_NO_WORKSPACE:
+            workspace = torch.empty(have, dtype=torch.uint8, device="cuda")
+            at = workspace.data_ptr()
+    _lib.check_spine(getattr(lib, name)(ref, at, have, stream_handle()), name)
 
 
 def linear(weights: torch.Tensor, x: torch.Tensor, bias: torch.Tensor | None = None,
@@ -102,34 +116,22 @@ def linear(weights: torch.Tensor, x: torch.Tensor, bias: torch.Tensor | None = N
     output's dtype, and may be `out` itself.  out_dtype: x's unless given.  Sums are fp32
     and rounded once.  workspace: uint8, at least linear_workspace's bytes, for a caller
     that keeps one (one per call that may run at the same time)."""
-    d, out = _linear_descriptor(weights, x, bias, activation, residual, row_scales, out_dtype, out)
-    _run("k3_hip_linear", d, workspace)
-    return out
-
-
-def _linear_descriptor(weights, x, bias, activation, residual, row_scales, out_dtype, out):
     kind = _matrix(weights, row_scales, "weights")
     rows, cols = weights.shape
     x2 = _rows(x, cols, "x")
     if activation not in ACTIVATIONS:
         raise ValueError(f"activation must be None, 'silu' or 'gelu', got {activation!r}")
-    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
-    if dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"outputs are float32 or bfloat16, not {dtype}")
-    shape = (x2.shape[0], rows)
+    out = _out(out, x2, rows, out_dtype)
     if bias is not None:
         _check(bias, torch.float32, (rows,), "bias")
     if residual is not None:
-        _check(residual, dtype, shape, "residual")
-    out = _out(out, shape, dtype, "out")
-    d = _lib.K3HipLinearV1()
-    d.abi_version, d.struct_bytes = _lib.K3_DENSE_ABI_V1, C.sizeof(d)
-    d.matrix_kind, d.activation = kind, ACTIVATIONS[activation]
-    d.x_dtype, d.out_dtype = _dtype_code(x2), _dtype_code(out)
-    d.rows, d.columns, d.positions = rows, cols, x2.shape[0]
-    d.weights, d.row_scales, d.bias = _ptr(weights), _ptr(row_scales), _ptr(bias)
-    d.x, d.residual, d.out = _ptr(x2), _ptr(residual), _ptr(out)
-    return d, out
+        _check(residual, out.dtype, out.shape, "residual")
+    d = _lib.K3HipLinearV1(
+        _lib.K3_DENSE_ABI_V1, C.sizeof(_lib.K3HipLinearV1), kind, ACTIVATIONS[activation],
+        _dtype_code(x2), _dtype_code(out), rows, cols, x2.shape[0], 0, weights.data_ptr(),
+        _ptr(row_scales), _ptr(bias), x2.data_ptr(), _ptr(residual), out.data_ptr())
+    _run("k3_hip_linear", d, workspace)
+    return out
 
 
 def _gate_code(activation) -> int:
@@ -163,21 +165,13 @@ def gated_ffn(w_gate: torch.Tensor, w_up: torch.Tensor, x: torch.Tensor,
     rows, cols = w_gate.shape
     x2 = _rows(x, cols, "x")
     code = _gate_code(activation)
-    dtype = out_dtype or (out.dtype if out is not None else x.dtype)
-    if dtype not in (torch.float32, torch.bfloat16):
-        raise ValueError(f"outputs are float32 or bfloat16, not {dtype}")
-    shape = (x2.shape[0], rows)
-    out = _out(out, shape, dtype, "out")
+    out = _out(out, x2, rows, out_dtype)
     g = torch.empty_like(out) if keep else None
     u = torch.empty_like(out) if keep else None
-    d = _lib.K3HipGatedV1()
-    d.abi_version, d.struct_bytes = _lib.K3_DENSE_ABI_V1, C.sizeof(d)
-    d.matrix_kind, d.activation = kind, code
-    d.x_dtype, d.out_dtype = _dtype_code(x2), _dtype_code(out)
-    d.rows, d.columns, d.positions = rows, cols, x2.shape[0]
-    d.gate, d.up = _ptr(w_gate), _ptr(w_up)
-    d.gate_scales, d.up_scales = _ptr(gate_scales), _ptr(up_scales)
-    d.x, d.out, d.out_gate, d.out_up = _ptr(x2), _ptr(out), _ptr(g), _ptr(u)
+    d = _lib.K3HipGatedV1(
+        _lib.K3_DENSE_ABI_V1, C.sizeof(_lib.K3HipGatedV1), kind, code, _dtype_code(x2),
+        _dtype_code(out), rows, cols, x2.shape[0], 0, w_gate.data_ptr(), w_up.data_ptr(),
+        _ptr(gate_scales), _ptr(up_scales), x2.data_ptr(), out.data_ptr(), _ptr(g), _ptr(u))
     _run("k3_hip_gated_ffn", d, workspace)
     return (out, g, u) if keep else out
 
@@ -201,14 +195,11 @@ def gated_ffn_backward(w_gate: torch.Tensor, w_up: torch.Tensor, x: torch.Tensor
     for t, name in zip(two, ("g", "u", "grad")):
         _check(t, x2.dtype, shape, name)
     d_x = torch.empty_like(x2)
-    d_gate = torch.empty(rows, cols, dtype=x2.dtype, device="cuda")
+    d_gate = torch.empty((rows, cols), dtype=x2.dtype, device=x2.device)
     d_up = torch.empty_like(d_gate)
-    d = _lib.K3HipGatedGradV1()
-    d.abi_version, d.struct_bytes = _lib.K3_DENSE_ABI_V1, C.sizeof(d)
-    d.activation, d.dtype = code, _dtype_code(x2)
-    d.rows, d.columns, d.positions = rows, cols, x2.shape[0]
-    d.gate, d.up, d.x = _ptr(w_gate), _ptr(w_up), _ptr(x2)
-    d.g, d.u, d.grad = (_ptr(t) for t in two)
-    d.d_x, d.d_gate, d.d_up = _ptr(d_x), _ptr(d_gate), _ptr(d_up)
+    d = _lib.K3HipGatedGradV1(
+        _lib.K3_DENSE_ABI_V1, C.sizeof(_lib.K3HipGatedGradV1), code, _dtype_code(x2), rows, cols,
+        x2.shape[0], 0, w_gate.data_ptr(), w_up.data_ptr(), x2.data_ptr(),
+        *(t.data_ptr() for t in two), d_x.data_ptr(), d_gate.data_ptr(), d_up.data_ptr())
     _run("k3_hip_gated_ffn_grad", d, workspace)
     return d_x, d_gate, d_up

@@ -43,12 +43,12 @@ def sample(logits: torch.Tensor, u: torch.Tensor, temperature: torch.Tensor | No
         if t is not None:
             _check(t, dtype, (rows,), name)
     if out is None:
-        out = torch.empty(rows, dtype=torch.int32, device="cuda")
-    _check(out, torch.int32, (rows,), "out")
-    d = _lib.K3HipSampleV1()
-    d.abi_version, d.struct_bytes = _lib.K3_SAMPLE_ABI_V1, C.sizeof(d)
-    d.logits_dtype, d.rows, d.vocabulary = _dtype_code(logits), rows, vocab
-    d.logits, d.u, d.temperature = _ptr(logits), _ptr(u), _ptr(temperature)
-    d.top_k, d.top_p, d.min_p, d.tokens = _ptr(top_k), _ptr(top_p), _ptr(min_p), _ptr(out)
+        out = torch.empty(rows, dtype=torch.int32, device=logits.device)
+    else:
+        _check(out, torch.int32, (rows,), "out")
+    d = _lib.K3HipSampleV1(
+        _lib.K3_SAMPLE_ABI_V1, C.sizeof(_lib.K3HipSampleV1), _dtype_code(logits), rows, vocab, 0,
+        logits.data_ptr(), u.data_ptr(), _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p),
+        out.data_ptr())
     _run("k3_hip_sample", d, workspace)
     return out

@@ -23,7 +23,8 @@
  *     output itself;
  *   - scratch memory is the caller's: the matching *_workspace_bytes gives its size for
  *     a descriptor (0 with a reason for an invalid one; pointers count by their
- *     alignment only, NULL as an aligned one where the operand is not optional).  The
+ *     alignment only, NULL as an aligned one where the operand is not optional).  A size
+ *     of K3_DENSE_NO_WORKSPACE means that the call uses none and takes NULL as well.  The
  *     workspace is 256-byte aligned and holds nothing between calls.  Calls that may
  *     run at the same time, replays of captured graphs among them, need one each.
  * rows, columns and positions are 1..1048576.
@@ -47,6 +48,7 @@ extern "C" {
 
 #define K3_DENSE_ABI_V1 1u
 #define K3_DENSE_MAX_EXTENT 1048576u /* of rows, columns and positions */
+#define K3_DENSE_NO_WORKSPACE 256u   /* size of a call that uses no scratch memory */
 
 /* Activation of a projection: z, z / (1 + exp(-z)), z / 2 (1 + erf(z / sqrt 2)). */
 enum { K3_DENSE_ACT_NONE = 0, K3_DENSE_ACT_SILU = 1, K3_DENSE_ACT_GELU = 2 };

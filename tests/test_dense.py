@@ -97,14 +97,26 @@ def test_grad_refusals(kw, match):
 def test_workspace_refusals(name, make):
     from deltafin_amd import _lib
     lib = _lib.load()
-    need = getattr(lib, name + "_workspace_bytes")(C.byref(make()))
-    assert need >= 256
-    _refused(name, make(), "workspace", ws=None)
-    _refused(name, make(), "workspace", ws=256 * A + 16)
-    _refused(name, make(), "workspace", bytes_=need - 1)
+    need = getattr(lib, name + "_workspace_bytes")(C.byref(make(positions=50)))
+    assert need > _lib.K3_DENSE_NO_WORKSPACE
+    _refused(name, make(positions=50), "workspace", ws=None)
+    _refused(name, make(positions=50), "workspace", ws=256 * A + 16)
+    _refused(name, make(positions=50), "workspace", bytes_=need - 1)
     _refused(name, None, "null descriptor")
     assert getattr(lib, name + "_workspace_bytes")(None) == 0
     assert getattr(lib, name + "_workspace_bytes")(C.byref(make(rows=0))) == 0
+
+
+def test_a_small_workspace_is_not_none():
+    """The smallest scratch memory there is (one row's dg and du) is told from none at all."""
+    from deltafin_amd import _lib
+    lib = _lib.load()
+    d = _grad(rows=8, columns=16, positions=1, dtype=_lib.K3_DTYPE_BF16)
+    assert lib.k3_hip_gated_ffn_grad_workspace_bytes(C.byref(d)) > _lib.K3_DENSE_NO_WORKSPACE
+    _refused("k3_hip_gated_ffn_grad", d, "workspace", ws=None,
+             bytes_=_lib.K3_DENSE_NO_WORKSPACE)
+    none = _linear(x_dtype=_lib.K3_DTYPE_BF16, positions=1)
+    assert (lib.k3_hip_linear_workspace_bytes(C.byref(none)) == _lib.K3_DENSE_NO_WORKSPACE)
 
 
 def test_workspace_counts_what_is_laid_out_again():
@@ -114,7 +126,7 @@ def test_workspace_counts_what_is_laid_out_again():
     size = lambda **kw: lib.k3_hip_linear_workspace_bytes(C.byref(_linear(
         rows=65536, columns=64, positions=4096, **kw)))
     bf16 = _lib.K3_DTYPE_BF16
-    assert size(x_dtype=bf16) == 256
+    assert size(x_dtype=bf16) == _lib.K3_DENSE_NO_WORKSPACE
     assert size(x_dtype=bf16, x=2 * A + 2) >= 4096 * 64 * 2
     assert size() >= 3 * 4096 * 64 * 2
     assert size(x_dtype=bf16, weights=A + 2) >= 65536 * 64 * 2
