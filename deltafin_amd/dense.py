@@ -30,7 +30,8 @@ GATES = {"situ": _lib.K3_ACT_SITU, "silu": _lib.K3_ACT_SILU}
 def _check(t: torch.Tensor, dtypes, shape, what: str) -> None:
     """t is a contiguous tensor of one of the dtypes and the shape on the current device.
     (One comparison after the other on purpose: a decode step's call is host bound.)"""
-    if (t.dtype is dtypes or t.dtype in dtypes) and t.shape == shape and t.is_contiguous():
+    fits = t.dtype in dtypes if isinstance(dtypes, tuple) else t.dtype is dtypes
+    if fits and t.shape == shape and t.is_contiguous():
         at = t.get_device()
         if at >= 0:
             if at == torch.cuda.current_device():
