@@ -1,17 +1,20 @@
 // Token sampling (include/k3_hip_sample_abi.h) by selection instead of sorting.
 //
 // Every limit of a row (top-k, top-p, min-p) and the draw itself is a position in one
-// order of its tokens, and a position is found by a radix descent over the 32-bit keys of
-// the logits: a histogram of token counts and weight sums over the top 11 key bits, the
-// bin in which the count or the sum crosses the wanted one, then the next 11 bits of that
-// bin's tokens and the last 10.  Nothing is sorted or written back, so the work is a few
-// reads of the row.
+// order of its tokens.  A position is found in two steps: in a histogram of token counts
+// and weight sums over 2048 equal ranges of the logit, from the row's largest down to
+// where weights vanish (or its smallest), the range in which the count or the sum crosses
+// the wanted one; then, among that range's tokens, by their keys eight bits at a time, and
+// by index among equal ones.  Nothing is sorted or written back.
 //
 // Weights are 64-bit integers (see fixed_weight): sums of them are exact, so LDS and
-// global atomics may add in any order, and two workgroups' histograms join without one.
+// global atomics may add in any order, and workgroups' histograms join without one.
 //
-// Launches: the row maxima (which the weights need), the first histogram (both over many
-// workgroups per row), and one workgroup per row for the descents.
+// Launches: the rows' largest and smallest logits, the histogram (both over many
+// workgroups per row), and one workgroup per row for the positions.  That one reads its
+// row once more: it gathers the tokens from the top through the first range it needs, up
+// to kList of them, in LDS, and most often every position lies among them.  A range that
+// does not fit (thousands of near-equal logits) is walked in memory instead.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -25,9 +28,11 @@
 namespace k3 {
 namespace {
 
-constexpr int kBins = 2048;          // of the first and second digit
+constexpr int kBins = 2048;          // of the first histogram
+constexpr int kList = 4096;          // tokens that the last workgroup holds
 constexpr int kScanThreads = 256;    // of the passes over a row's parts
 constexpr int kPickThreads = 1024;   // of the workgroup that ends a row
+constexpr double kVanish = 64.0;     // weights under 2^-kVanish round to none
 
 struct SampleArgs {
   const void* logits;
@@ -37,7 +42,7 @@ struct SampleArgs {
   const float* top_p;
   const float* min_p;
   int32_t* tokens;
-  uint32_t* part_max;  // [rows][parts] keys of the parts' largest logits
+  uint32_t* ends;      // [rows][parts][2] keys of the parts' largest and smallest logits
   uint32_t* count;     // [rows][kBins]
   uint64_t* mass;      // [rows][kBins]
   int rows, vocab, parts, part;  // parts of a row and tokens of one
@@ -60,15 +65,22 @@ constexpr uint32_t kKeyMasked = 0xff800000u;  // of -inf
 struct RowParams {
   float top;       // largest logit
   double rate;     // log2(e) / T; 0 where only the largest logits weigh
+  double per_bin;  // bins per halving of the weight
   bool sampled;    // T > 0
 };
 
-__device__ __forceinline__ RowParams row_params(const SampleArgs& a, int row, uint32_t top_key) {
+__device__ __forceinline__ double log2_weight(const RowParams& r, float l);
+
+// bottom_key: of the smallest logit over -inf.
+__device__ __forceinline__ RowParams row_params(const SampleArgs& a, int row, uint32_t top_key,
+                                                uint32_t bottom_key) {
   RowParams r;
   r.top = value_of(top_key);
   const float t = a.temperature ? a.temperature[row] : 1.f;
   r.sampled = t > 0.f;
   r.rate = r.sampled ? 1.4426950408889634 / (double)t : 0.0;
+  const double range = -log2_weight(r, value_of(bottom_key));
+  r.per_bin = range > 0.0 ? (double)(kBins - 2) / fmin(range, kVanish) : 0.0;
   return r;
 }
 
@@ -79,12 +91,16 @@ __device__ __forceinline__ double log2_weight(const RowParams& r, float l) {
   return ((double)l - (double)r.top) * r.rate;
 }
 
-// Weight times 2^shift, to the nearest integer: 2^y by y = n + h / 64 + f with |f| <= 1 / 128,
+// The bin of a token of log2 weight y: it never falls as y does; the last one holds what
+// weighs nothing.
+__device__ __forceinline__ int bin_of(const RowParams& r, double y) {
+  return y > -kVanish ? min((int)(-y * r.per_bin), kBins - 2) : kBins - 1;
+}
+
+// 2^y times 2^shift, to the nearest integer: y = n + h / 64 + f with |f| <= 1 / 128,
 // 2^(h / 64) from LDS and 2^f by its Taylor series (the first term left out is under 2^-52).
-__device__ __forceinline__ uint64_t fixed_weight(const RowParams& r, const double* table, int shift,
-                                                 float l) {
-  const double y = log2_weight(r, l);
-  if (!(y > -64.0)) return 0;
+__device__ __forceinline__ uint64_t fixed_weight(const double* table, int shift, double y) {
+  if (!(y > -kVanish)) return 0;
   const double q = rint(y * 64.0);
   const double f = (y - q * 0.015625) * 0.6931471805599453;  // times ln 2
   const int qi = (int)q;
@@ -149,20 +165,54 @@ __device__ __forceinline__ uint32_t wave_min(uint32_t v) {
   return v;
 }
 
+// The keys of a row's largest logit and of its smallest over -inf (0 where there is none),
+// from every thread's own; red is shared, 2 words per wave.
+__device__ __forceinline__ void block_ends(uint32_t* red, int waves, uint32_t* top,
+                                           uint32_t* bottom) {
+  const uint32_t t = wave_min(*top), b = ~wave_min(~*bottom);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) {
+    red[2 * (threadIdx.x >> 6)] = t;
+    red[2 * (threadIdx.x >> 6) + 1] = b;
+  }
+  __syncthreads();
+  *top = red[0];
+  *bottom = red[1];
+  for (int w = 1; w < waves; ++w) {
+    *top = min(*top, red[2 * w]);
+    *bottom = max(*bottom, red[2 * w + 1]);
+  }
+}
+
+__device__ __forceinline__ void row_ends(const SampleArgs& a, int row, uint32_t* red, int threads,
+                                         uint32_t* top, uint32_t* bottom) {
+  *top = 0xffffffffu;
+  *bottom = 0u;
+  for (int i = threadIdx.x; i < a.parts; i += threads) {
+    const uint32_t* e = a.ends + 2 * ((uint64_t)row * a.parts + i);
+    *top = min(*top, e[0]);
+    *bottom = max(*bottom, e[1]);
+  }
+  block_ends(red, threads / 64, top, bottom);
+}
+
 template <typename T>
-__global__ __launch_bounds__(kScanThreads) void k_sample_max(const SampleArgs a) {
+__global__ __launch_bounds__(kScanThreads) void k_sample_ends(const SampleArgs a) {
   const int row = blockIdx.y, part = blockIdx.x;
-  uint32_t best = 0xffffffffu;
+  uint32_t top = 0xffffffffu, bottom = 0u;
   const int t0 = part * a.part, t1 = min(t0 + a.part, a.vocab);
   scan(static_cast<const T*>(a.logits) + (uint64_t)row * a.vocab, t0, t1, kScanThreads,
-       [&](float l, int) { best = min(best, key_of(l)); });
-  best = wave_min(best);
-  __shared__ uint32_t red[kScanThreads / 64];
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = best;
-  __syncthreads();
+       [&](float l, int) {
+         const uint32_t k = key_of(l);
+         top = min(top, k);
+         bottom = max(bottom, k == kKeyMasked ? 0u : k);
+       });
+  __shared__ uint32_t red[2 * kScanThreads / 64];
+  block_ends(red, kScanThreads / 64, &top, &bottom);
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kScanThreads / 64; ++w) best = min(best, red[w]);
-    a.part_max[(uint64_t)row * a.parts + part] = best;
+    uint32_t* e = a.ends + 2 * ((uint64_t)row * a.parts + part);
+    e[0] = top;
+    e[1] = bottom;
   }
   // this part's share of the row's histogram, for the next launch to add to
   for (int b = part * kScanThreads + threadIdx.x; b < kBins; b += a.parts * kScanThreads) {
@@ -171,31 +221,31 @@ __global__ __launch_bounds__(kScanThreads) void k_sample_max(const SampleArgs a)
   }
 }
 
-__device__ __forceinline__ uint32_t row_top(const SampleArgs& a, int row) {
-  uint32_t best = 0xffffffffu;
-  for (int i = 0; i < a.parts; ++i) best = min(best, a.part_max[(uint64_t)row * a.parts + i]);
-  return best;
-}
-
 template <typename T>
 __global__ __launch_bounds__(kScanThreads) void k_sample_histogram(const SampleArgs a) {
   const int row = blockIdx.y, part = blockIdx.x;
   __shared__ uint32_t count[kBins];
   __shared__ uint64_t mass[kBins];
   __shared__ double table[64];
+  __shared__ uint32_t red[2 * kScanThreads / 64];
   fill_table(table);
   for (int b = threadIdx.x; b < kBins; b += kScanThreads) {
     count[b] = 0;
     mass[b] = 0;
   }
-  const RowParams r = row_params(a, row, row_top(a, row));
+  uint32_t top, bottom;
+  row_ends(a, row, red, kScanThreads, &top, &bottom);
+  const RowParams r = row_params(a, row, top, bottom);
+  if (top == kKeyMasked || !r.sampled) return;  // the last launch needs no histogram
   __syncthreads();
   const int t0 = part * a.part, t1 = min(t0 + a.part, a.vocab);
   scan(static_cast<const T*>(a.logits) + (uint64_t)row * a.vocab, t0, t1, kScanThreads,
        [&](float l, int) {
-         const uint32_t b = key_of(l) >> 21;
+         if (l != l) l = -INFINITY;
+         const double y = log2_weight(r, l);
+         const int b = bin_of(r, y);
          atomicAdd(&count[b], 1u);
-         const uint64_t w = fixed_weight(r, table, a.shift, l);
+         const uint64_t w = fixed_weight(table, a.shift, y);
          if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&mass[b]), (unsigned long long)w);
        });
   __syncthreads();
@@ -208,254 +258,342 @@ __global__ __launch_bounds__(kScanThreads) void k_sample_histogram(const SampleA
   }
 }
 
-// A position in a row's order: the key of its token and what lies before that key.
-struct Found {
-  uint32_t key;
-  uint32_t before;       // tokens of smaller keys
-  uint64_t mass_before;  // and their weight
-  uint32_t equal;        // tokens of this key
-};
-
 struct PickShared {
-  uint32_t count[kBins];
+  uint32_t count[kBins];  // running counts and masses, each bin's own included
   uint64_t mass[kBins];
   double table[64];
+  uint32_t digit_count[256];
+  uint64_t digit_mass[256];
+  uint32_t key[kList];
+  int32_t index[kList];
+  uint32_t listed;
   uint32_t wave_count[kPickThreads / 64];
   uint64_t wave_mass[kPickThreads / 64];
-  uint32_t bin, before;
+  uint32_t red[2 * kPickThreads / 64];
+  int bin;
+  uint32_t digit, before;
   uint64_t mass_before;
-  int token;
 };
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
   return (uint64_t)__shfl_up((unsigned long long)v, d);
 }
+__device__ __forceinline__ void add64(uint64_t* to, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(to), (unsigned long long)v);
+}
 
-// The first bin of sh.count / sh.mass at which the running count (by_count) or mass,
-// `before` included, exceeds `target`: into sh.bin, sh.before and sh.mass_before.  There
-// is one.
-__device__ __forceinline__ void cross(PickShared& sh, int bins, bool by_count, uint64_t target,
-                                      uint32_t before, uint64_t mass_before) {
-  const int b = 2 * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t c0 = b < bins ? sh.count[b] : 0u, c1 = b < bins ? sh.count[b + 1] : 0u;
-  const uint64_t m0 = b < bins ? sh.mass[b] : 0u, m1 = b < bins ? sh.mass[b + 1] : 0u;
-  uint32_t c = c0 + c1;
-  uint64_t m = m0 + m1;
+// A position in a row's order: the key of its token and what lies before that key.
+struct Found {
+  uint32_t key;
+  uint32_t before;       // tokens of smaller keys
+  uint64_t mass_before;  // and their weight
+};
+
+// One row's workgroup.  Every member is called by all of its threads.
+template <typename T>
+struct Picker {
+  PickShared& sh;
+  const SampleArgs& a;
+  const T* row;
+  RowParams r;
+  int first = 0, last = -1;  // bins whose tokens are listed
+
+  // The histogram, as running sums.
+  __device__ __forceinline__ void load_histogram(int row_index) {
+    const int b = 2 * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t* gc = a.count + (uint64_t)row_index * kBins;
+    const uint64_t* gm = a.mass + (uint64_t)row_index * kBins;
+    const uint32_t c0 = gc[b], c1 = gc[b + 1];
+    const uint64_t m0 = gm[b], m1 = gm[b + 1];
+    uint32_t c = c0 + c1;
+    uint64_t m = m0 + m1;
 #pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const uint32_t cu = __shfl_up(c, d);
-    const uint64_t mu = shfl_up64(m, d);
-    if (lane >= d) {
-      c += cu;
-      m += mu;
-    }
-  }
-  if (lane == 63) {
-    sh.wave_count[wave] = c;
-    sh.wave_mass[wave] = m;
-  }
-  __syncthreads();
-  c += before;
-  m += mass_before;
-  for (int w = 0; w < wave; ++w) {
-    c += sh.wave_count[w];
-    m += sh.wave_mass[w];
-  }
-  // running values ahead of this thread's two bins, between them and behind them
-  const uint32_t r0 = c - c0 - c1, r1 = c - c1;
-  const uint64_t s0 = m - m0 - m1, s1 = m - m1;
-  const uint64_t v0 = by_count ? r0 : s0, v1 = by_count ? r1 : s1, v2 = by_count ? c : m;
-  if (v0 <= target && v1 > target) {
-    sh.bin = b;
-    sh.before = r0;
-    sh.mass_before = s0;
-  } else if (v1 <= target && v2 > target) {
-    sh.bin = b + 1;
-    sh.before = r1;
-    sh.mass_before = s1;
-  }
-  __syncthreads();
-}
-
-// The histogram of the digit of `bits` key bits above `low`, over the row's tokens whose
-// higher bits are `prefix`.
-template <typename T>
-__device__ __forceinline__ void digit_histogram(PickShared& sh, const SampleArgs& a, const T* row,
-                                                const RowParams& r, uint32_t prefix, int low,
-                                                int bits) {
-  __syncthreads();
-  for (int b = threadIdx.x; b < (1 << bits); b += kPickThreads) {
-    sh.count[b] = 0;
-    sh.mass[b] = 0;
-  }
-  __syncthreads();
-  scan(row, 0, a.vocab, kPickThreads, [&](float l, int) {
-    const uint32_t k = key_of(l);
-    if (k >> (low + bits) != prefix) return;
-    const uint32_t b = (k >> low) & ((1u << bits) - 1u);
-    atomicAdd(&sh.count[b], 1u);
-    const uint64_t w = fixed_weight(r, sh.table, a.shift, l);
-    if (w) atomicAdd(reinterpret_cast<unsigned long long*>(&sh.mass[b]), (unsigned long long)w);
-  });
-  __syncthreads();
-}
-
-__device__ __forceinline__ void first_histogram(PickShared& sh, const SampleArgs& a, int row) {
-  __syncthreads();
-  for (int b = threadIdx.x; b < kBins; b += kPickThreads) {
-    sh.count[b] = a.count[(uint64_t)row * kBins + b];
-    sh.mass[b] = a.mass[(uint64_t)row * kBins + b];
-  }
-  __syncthreads();
-}
-
-// The first token of the order at which the running count or mass exceeds target.
-template <typename T>
-__device__ __forceinline__ Found descend(PickShared& sh, const SampleArgs& a, int row_index,
-                                         const T* row, const RowParams& r, bool by_count,
-                                         uint64_t target) {
-  first_histogram(sh, a, row_index);
-  cross(sh, kBins, by_count, target, 0u, 0u);
-  uint32_t prefix = sh.bin, before = sh.before;
-  uint64_t mass_before = sh.mass_before;
-  digit_histogram(sh, a, row, r, prefix, 10, 11);
-  cross(sh, 2048, by_count, target, before, mass_before);
-  prefix = prefix << 11 | sh.bin;
-  before = sh.before;
-  mass_before = sh.mass_before;
-  digit_histogram(sh, a, row, r, prefix, 0, 10);
-  cross(sh, 1024, by_count, target, before, mass_before);
-  Found f;
-  f.key = prefix << 10 | sh.bin;
-  f.before = sh.before;
-  f.mass_before = sh.mass_before;
-  f.equal = sh.count[sh.bin];
-  __syncthreads();
-  return f;
-}
-
-// The token of rank `nth` (from 0) among those with the key, by index.
-template <typename T>
-__device__ __forceinline__ int nth_equal(PickShared& sh, const SampleArgs& a, const T* row,
-                                         uint32_t key, uint32_t nth) {
-  constexpr int kWaves = kPickThreads / 64;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int share = (a.vocab + kWaves - 1) / kWaves;
-  const int t0 = min(wave * share, a.vocab), t1 = min(t0 + share, a.vocab);
-  auto is = [&](int t) {
-    if (t >= t1) return false;
-    float l;
-    if constexpr (sizeof(T) == 4)
-      l = row[t];
-    else
-      l = bf16_bits_to_f32(row[t]);
-    return key_of(l) == key;
-  };
-  uint32_t n = 0;
-  for (int t = t0; t < t1; t += 64) n += __popcll(__ballot(is(t + lane)));
-  if (lane == 0) sh.wave_count[wave] = n;
-  __syncthreads();
-  uint32_t before = 0;
-  for (int w = 0; w < wave; ++w) before += sh.wave_count[w];
-  if (before <= nth && nth < before + n) {
-    uint32_t left = nth - before;
-    for (int t = t0; t < t1; t += 64) {
-      const bool here = is(t + lane);
-      const uint64_t mask = __ballot(here);
-      const uint32_t m = (uint32_t)__popcll(mask);
-      if (left < m) {
-        if (here && (uint32_t)__popcll(mask & ((1ull << lane) - 1)) == left) sh.token = t + lane;
-        break;
+    for (int d = 1; d < 64; d <<= 1) {
+      const uint32_t cu = __shfl_up(c, d);
+      const uint64_t mu = shfl_up64(m, d);
+      if (lane >= d) {
+        c += cu;
+        m += mu;
       }
-      left -= m;
+    }
+    if (lane == 63) {
+      sh.wave_count[wave] = c;
+      sh.wave_mass[wave] = m;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+      c += sh.wave_count[w];
+      m += sh.wave_mass[w];
+    }
+    sh.count[b] = c - c1;
+    sh.count[b + 1] = c;
+    sh.mass[b] = m - m1;
+    sh.mass[b + 1] = m;
+    __syncthreads();
+  }
+
+  // The first bin whose running count or mass exceeds target; there is one.
+  __device__ __forceinline__ int crossing(bool by_count, uint64_t target) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int b = 2 * threadIdx.x + i;
+      const uint64_t here = by_count ? sh.count[b] : sh.mass[b];
+      const uint64_t ahead = b == 0 ? 0 : by_count ? sh.count[b - 1] : sh.mass[b - 1];
+      if (ahead <= target && here > target) sh.bin = b;
+    }
+    __syncthreads();
+    return sh.bin;
+  }
+
+  __device__ __forceinline__ uint32_t count_before(int bin) const {
+    return bin ? sh.count[bin - 1] : 0u;
+  }
+  __device__ __forceinline__ uint64_t mass_before(int bin) const {
+    return bin ? sh.mass[bin - 1] : 0u;
+  }
+
+  // Lists the tokens of the bin, with those of every larger logit where they fit.
+  __device__ __forceinline__ void list(int bin) {
+    if (first <= bin && bin <= last) return;
+    const int from = sh.count[bin] <= (uint32_t)kList ? 0 : bin;
+    if (sh.count[bin] - count_before(from) > (uint32_t)kList) return;  // stays in memory
+    __syncthreads();
+    if (threadIdx.x == 0) sh.listed = 0;
+    __syncthreads();
+    scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
+      if (l != l) l = -INFINITY;
+      const int b = bin_of(r, log2_weight(r, l));
+      if (b < from || b > bin) return;
+      const uint32_t at = atomicAdd(&sh.listed, 1u);
+      if (at >= (uint32_t)kList) return;  // the row changed under the call
+      sh.key[at] = key_of(l);
+      sh.index[at] = t;
+    });
+    __syncthreads();
+    first = from;
+    last = bin;
+  }
+
+  // Calls f(key, index, log2 weight) for the bin's tokens, each thread its share.
+  template <typename F>
+  __device__ __forceinline__ void each(int bin, F f) {
+    if (first <= bin && bin <= last) {
+      const int n = min((int)sh.listed, kList);
+      for (int i = threadIdx.x; i < n; i += kPickThreads) {
+        const double y = log2_weight(r, value_of(sh.key[i]));
+        if (bin_of(r, y) == bin) f(sh.key[i], sh.index[i], y);
+      }
+    } else {
+      scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
+        if (l != l) l = -INFINITY;
+        const double y = log2_weight(r, l);
+        if (bin_of(r, y) == bin) f(key_of(l), t, y);
+      });
     }
   }
-  __syncthreads();
-  return sh.token;
-}
+
+  // Of the 256 digits, the first at which the running count or mass (what lies before the
+  // digits included) exceeds target: into sh.digit, sh.before and sh.mass_before.
+  __device__ __forceinline__ void cross_digit(bool by_count, uint64_t target, uint32_t before,
+                                              uint64_t mass) {
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      uint32_t c[4];
+      uint64_t m[4];
+      uint32_t cs = 0;
+      uint64_t ms = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        c[i] = sh.digit_count[4 * threadIdx.x + i];
+        m[i] = sh.digit_mass[4 * threadIdx.x + i];
+        cs += c[i];
+        ms += m[i];
+      }
+      uint32_t ci = cs;
+      uint64_t mi = ms;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t cu = __shfl_up(ci, d);
+        const uint64_t mu = shfl_up64(mi, d);
+        if ((int)threadIdx.x >= d) {
+          ci += cu;
+          mi += mu;
+        }
+      }
+      uint32_t cr = before + ci - cs;
+      uint64_t mr = mass + mi - ms;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint64_t ahead = by_count ? cr : mr;
+        const uint64_t here = by_count ? (uint64_t)(cr + c[i]) : mr + m[i];
+        if (ahead <= target && here > target) {
+          sh.digit = 4 * threadIdx.x + i;
+          sh.before = cr;
+          sh.mass_before = mr;
+        }
+        cr += c[i];
+        mr += m[i];
+      }
+    }
+    __syncthreads();
+  }
+
+  __device__ __forceinline__ void clear_digits() {
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      sh.digit_count[threadIdx.x] = 0;
+      sh.digit_mass[threadIdx.x] = 0;
+    }
+    __syncthreads();
+  }
+
+  // The bits in which the values that `walk` shows differ, from the highest differing one
+  // down; their common part goes to *common.
+  template <typename W>
+  __device__ __forceinline__ int differing_bits(W walk, uint32_t* common) {
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    walk([&](uint32_t v, double) {
+      lo = min(lo, v);
+      hi = max(hi, v);
+    });
+    block_ends(sh.red, kPickThreads / 64, &lo, &hi);
+    const uint32_t x = lo ^ hi;
+    const int bits = x ? 32 - __clz((int)x) : 0;
+    *common = bits == 32 ? 0u : lo >> bits << bits;
+    return bits;
+  }
+
+  // The value, among those that `walk` shows with their log2 weights, at which the running
+  // count or mass exceeds target; before and mass lie ahead of all of them.
+  template <typename W>
+  __device__ __forceinline__ Found descend(W walk, bool by_count, bool weigh, uint64_t target,
+                                           uint32_t before, uint64_t mass) {
+    Found f;
+    int low = differing_bits(walk, &f.key);
+    f.before = before;
+    f.mass_before = mass;
+    while (low > 0) {
+      const int width = min(low, 8);
+      const int high = low;
+      low -= width;
+      clear_digits();
+      const uint32_t prefix = high == 32 ? 0u : f.key >> high;
+      walk([&](uint32_t v, double y) {
+        if (high < 32 && v >> high != prefix) return;
+        const uint32_t d = (v >> low) & ((1u << width) - 1u);
+        atomicAdd(&sh.digit_count[d], 1u);
+        const uint64_t w = weigh ? fixed_weight(sh.table, a.shift, y) : 0;
+        if (w) add64(&sh.digit_mass[d], w);
+      });
+      cross_digit(by_count, target, f.before, f.mass_before);
+      f.key |= sh.digit << low;
+      f.before = sh.before;
+      f.mass_before = sh.mass_before;
+    }
+    return f;
+  }
+
+  // The first token at which the row's running count or mass exceeds target.
+  __device__ __forceinline__ Found find(bool by_count, uint64_t target, int* bin_out) {
+    const int bin = crossing(by_count, target);
+    *bin_out = bin;
+    list(bin);
+    return descend(
+        [&](auto f) { each(bin, [&](uint32_t k, int, double y) { f(k, y); }); }, by_count, true,
+        target, count_before(bin), mass_before(bin));
+  }
+
+  // The index of rank nth (from 0) among the bin's tokens of a key.
+  __device__ __forceinline__ int nth_equal(int bin, uint32_t key, uint32_t nth) {
+    return (int)descend(
+               [&](auto f) {
+                 each(bin, [&](uint32_t k, int t, double y) {
+                   if (k == key) f((uint32_t)t, y);
+                 });
+               },
+               true, false, nth, 0u, 0u)
+        .key;
+  }
+
+  __device__ __forceinline__ uint64_t weight(uint32_t key) const {
+    return fixed_weight(sh.table, a.shift, log2_weight(r, value_of(key)));
+  }
+
+  __device__ __forceinline__ uint64_t block_sum(uint64_t m) {
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) m += (uint64_t)__shfl_xor((unsigned long long)m, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.wave_mass[threadIdx.x >> 6] = m;
+    __syncthreads();
+    m = 0;
+    for (int w = 0; w < kPickThreads / 64; ++w) m += sh.wave_mass[w];
+    return m;
+  }
+};
 
 template <typename T>
 __global__ __launch_bounds__(kPickThreads) void k_sample_pick(const SampleArgs a) {
   __shared__ PickShared sh;
   const int ri = blockIdx.x;
   const T* row = static_cast<const T*>(a.logits) + (uint64_t)ri * a.vocab;
-  const uint32_t top = row_top(a, ri);
+  uint32_t top, bottom;
+  row_ends(a, ri, sh.red, kPickThreads, &top, &bottom);
   if (top == kKeyMasked) {  // nothing but -inf and NaN
     if (threadIdx.x == 0) a.tokens[ri] = -1;
     return;
   }
-  fill_table(sh.table);
-  const RowParams r = row_params(a, ri, top);
-  if (!r.sampled) {
-    const int t = nth_equal(sh, a, row, top, 0u);
-    if (threadIdx.x == 0) a.tokens[ri] = t;
+  const RowParams r = row_params(a, ri, top, bottom);
+  if (!r.sampled) {  // the lowest index of the largest logit
+    int at = a.vocab;
+    scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
+      if (l == r.top) at = min(at, t);
+    });
+    uint32_t lo = (uint32_t)at, hi = 0u;
+    block_ends(sh.red, kPickThreads / 64, &lo, &hi);
+    if (threadIdx.x == 0) a.tokens[ri] = (int)lo;
     return;
   }
-  // the sum over the whole row, then the mass of the top-k prefix
-  first_histogram(sh, a, ri);
-  uint64_t total = 0;
-  {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    uint64_t m = sh.mass[2 * threadIdx.x] + sh.mass[2 * threadIdx.x + 1];
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m += (uint64_t)__shfl_xor((unsigned long long)m, d);
-    if (lane == 0) sh.wave_mass[wave] = m;
-    __syncthreads();
-    for (int w = 0; w < kPickThreads / 64; ++w) total += sh.wave_mass[w];
-    __syncthreads();
-  }
-  auto weight = [&](uint32_t key) { return fixed_weight(r, sh.table, a.shift, value_of(key)); };
-  uint64_t kept = total;  // weight of the shortest prefix so far
+  fill_table(sh.table);
+  Picker<T> p{sh, a, row, r};
+  p.load_histogram(ri);
+  int bin;
+  uint64_t kept = sh.mass[kBins - 1];  // weight of the shortest prefix so far
   const int k = a.top_k ? a.top_k[ri] : 0;
-  if (k > 0 && k < a.vocab) {
-    const Found f = descend(sh, a, ri, row, r, true, (uint64_t)(k - 1));
-    kept = f.mass_before + (uint64_t)((uint32_t)k - f.before) * weight(f.key);
+  // (a first k that ends among the tokens of no weight leaves the sum as it is)
+  if (k > 0 && k < a.vocab && (uint32_t)k <= sh.count[kBins - 2]) {
+    const Found f = p.find(true, (uint64_t)(k - 1), &bin);
+    kept = f.mass_before + (uint64_t)((uint32_t)k - f.before) * p.weight(f.key);
   }
-  const float p = a.top_p ? a.top_p[ri] : 1.f;
-  if (p < 1.f) {
-    // the first prefix with a sum of at least p times the top-k one's
-    const uint64_t want = max((uint64_t)1, (uint64_t)ceil(fmax((double)p, 0.0) * (double)kept));
-    const Found f = descend(sh, a, ri, row, r, false, want - 1);
-    const uint64_t w = weight(f.key);
+  const float top_p = a.top_p ? a.top_p[ri] : 1.f;
+  if (top_p < 1.f) {
+    // the first prefix with a sum of at least top_p times the top-k one's
+    const uint64_t want =
+        max((uint64_t)1, (uint64_t)ceil(fmax((double)top_p, 0.0) * (double)kept));
+    const Found f = p.find(false, want - 1, &bin);
+    const uint64_t w = p.weight(f.key);
     kept = min(kept, f.mass_before + (want - f.mass_before + w - 1) / w * w);
   }
-  const float mp = a.min_p ? a.min_p[ri] : 0.f;
-  if (mp > 0.f) {
-    // the last key whose weight is at least min_p, by halving over the keys from the top
-    const double least = log2(fmin((double)mp, 1.0));
-    uint32_t lo = top, hi = kKeyMasked;  // lo is kept, hi is not
-    while (hi - lo > 1) {
-      const uint32_t mid = lo + (hi - lo) / 2;
-      if (log2_weight(r, value_of(mid)) >= least)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    // weight of the tokens up to it: a sum over its bin behind the bins before
-    const uint32_t bin = lo >> 21;
-    first_histogram(sh, a, ri);
+  const float min_p = a.min_p ? a.min_p[ri] : 0.f;
+  if (min_p > 0.f) {
+    const double least = log2(fmin((double)min_p, 1.0));
+    bin = bin_of(r, least);
     uint64_t m = 0;
-    for (uint32_t b = threadIdx.x; b < bin; b += kPickThreads) m += sh.mass[b];
-    scan(row, 0, a.vocab, kPickThreads, [&](float l, int) {
-      const uint32_t key = key_of(l);
-      if (key >> 21 == bin && key <= lo) m += fixed_weight(r, sh.table, a.shift, l);
-    });
-#pragma unroll
-    for (int d = 32; d > 0; d >>= 1) m += (uint64_t)__shfl_xor((unsigned long long)m, d);
-    if ((threadIdx.x & 63) == 0) sh.wave_mass[threadIdx.x >> 6] = m;
-    __syncthreads();
-    m = 0;
-    for (int w = 0; w < kPickThreads / 64; ++w) m += sh.wave_mass[w];
-    __syncthreads();
-    kept = min(kept, m);
+    if (p.mass_before(bin) < kept) {  // else a shorter prefix is there already
+      p.list(bin);
+      p.each(bin, [&](uint32_t, int, double y) {
+        if (y >= least) m += fixed_weight(sh.table, a.shift, y);
+      });
+      kept = min(kept, p.mass_before(bin) + p.block_sum(m));
+    }
   }
   float u = a.u[ri];
   if (!(u < 1.f)) u = 1.f - 0x1p-24f;
   u = fmaxf(u, 0.f);
   const uint64_t target = min((uint64_t)((double)u * (double)kept), kept - 1);
-  const Found f = descend(sh, a, ri, row, r, false, target);
-  const uint32_t nth = (uint32_t)((target - f.mass_before) / weight(f.key));
-  const int t = nth_equal(sh, a, row, f.key, nth);
+  const Found f = p.find(false, target, &bin);
+  const uint32_t nth = (uint32_t)((target - f.mass_before) / p.weight(f.key));
+  const int t = p.nth_equal(bin, f.key, nth);
   if (threadIdx.x == 0) a.tokens[ri] = t;
 }
 
@@ -463,14 +601,14 @@ uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
 
 struct SampleLayout {
   int parts, part;
-  uint64_t count, mass, bytes;  // offsets of the histograms behind the part maxima
+  uint64_t count, mass, bytes;  // offsets of the histograms behind the parts' ends
   SampleLayout(int rows, int vocab) {
     // parts of at least 4096 tokens, about two workgroups per CU over all rows
     const int want = std::max(1, 512 / rows);
     parts = std::min(want, (vocab + 4095) / 4096);
     part = (vocab + parts - 1) / parts;
     parts = (vocab + part - 1) / part;
-    count = align256(4ull * rows * parts);
+    count = align256(8ull * rows * parts);
     mass = count + align256(4ull * rows * kBins);
     bytes = mass + align256(8ull * rows * kBins);
   }
@@ -514,7 +652,7 @@ int sample_launch(const SampleArgs& a, hipStream_t st) {
   for (int step = 0; step < 3; ++step) {
     TimedLaunch tl(KC_ROUTE, st);
     if (step == 0)
-      launch_timed(tl, k_sample_max<T>, grid, dim3(kScanThreads), 0, st, a);
+      launch_timed(tl, k_sample_ends<T>, grid, dim3(kScanThreads), 0, st, a);
     else if (step == 1)
       launch_timed(tl, k_sample_histogram<T>, grid, dim3(kScanThreads), 0, st, a);
     else
@@ -563,7 +701,7 @@ int k3_hip_sample(const K3HipSampleV1* op, void* workspace, uint64_t workspace_b
   a.top_p = op->top_p;
   a.min_p = op->min_p;
   a.tokens = op->tokens;
-  a.part_max = reinterpret_cast<uint32_t*>(ws);
+  a.ends = reinterpret_cast<uint32_t*>(ws);
   a.count = reinterpret_cast<uint32_t*>(ws + l.count);
   a.mass = reinterpret_cast<uint64_t*>(ws + l.mass);
   a.rows = (int)op->rows;
