@@ -29,7 +29,7 @@ namespace k3 {
 namespace {
 
 constexpr int kBins = 2048;          // of the first histogram
-constexpr int kList = 4096;          // tokens that the last workgroup holds
+constexpr int kList = 12288;         // tokens that the last workgroup holds: 96 KB of its LDS
 constexpr int kScanThreads = 256;    // of the passes over a row's parts
 constexpr int kPickThreads = 1024;   // of the workgroup that ends a row
 constexpr double kVanish = 64.0;     // weights under 2^-kVanish round to none
@@ -199,14 +199,14 @@ __device__ __forceinline__ void row_ends(const SampleArgs& a, int row, uint32_t*
 template <typename T>
 __global__ __launch_bounds__(kScanThreads) void k_sample_ends(const SampleArgs a) {
   const int row = blockIdx.y, part = blockIdx.x;
-  uint32_t top = 0xffffffffu, bottom = 0u;
+  float most = -INFINITY, least = INFINITY;  // fmaxf and fminf pass NaN by
   const int t0 = part * a.part, t1 = min(t0 + a.part, a.vocab);
   scan(static_cast<const T*>(a.logits) + (uint64_t)row * a.vocab, t0, t1, kScanThreads,
        [&](float l, int) {
-         const uint32_t k = key_of(l);
-         top = min(top, k);
-         bottom = max(bottom, k == kKeyMasked ? 0u : k);
+         most = fmaxf(most, l);
+         least = fminf(least, l == -INFINITY ? INFINITY : l);
        });
+  uint32_t top = key_of(most), bottom = most > -INFINITY ? key_of(least) : 0u;
   __shared__ uint32_t red[2 * kScanThreads / 64];
   block_ends(red, kScanThreads / 64, &top, &bottom);
   if (threadIdx.x == 0) {
@@ -298,6 +298,25 @@ struct Picker {
   RowParams r;
   int first = 0, last = -1;  // bins whose tokens are listed
 
+  // The last key of the bins up to `bin`: bins never fall along the keys.  64 keys at a
+  // time; with the two ends of a bin known, tokens are told by their keys alone, without
+  // the fp64 of bin_of (which took half of a pass over the row).
+  __device__ __forceinline__ uint32_t last_key(int bin) const {
+    if (bin < 0) return key_of(r.top) - 1;
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = key_of(r.top), hi = kKeyMasked;  // lo is in, hi is not
+    while (hi - lo > 1) {
+      const uint32_t step = (hi - lo - 1) / 64 + 1;
+      const uint32_t at = lo + (lane + 1) * step;
+      const bool in = at < hi && at > lo && bin_of(r, log2_weight(r, value_of(at))) <= bin;
+      const uint32_t n = (uint32_t)__popcll(__ballot(in));
+      const uint32_t next = lo + (n + 1) * step;
+      lo += n * step;
+      if (n < 64 && next > lo && next < hi) hi = next;
+    }
+    return lo;
+  }
+
   // The histogram, as running sums.
   __device__ __forceinline__ void load_histogram(int row_index) {
     const int b = 2 * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -353,42 +372,43 @@ struct Picker {
     return bin ? sh.mass[bin - 1] : 0u;
   }
 
-  // Lists the tokens of the bin, with those of every larger logit where they fit.
-  __device__ __forceinline__ void list(int bin) {
+  // Lists the tokens of the bin (keys up to `to`), with those of every larger logit where
+  // they fit.
+  __device__ __forceinline__ void list(int bin, uint32_t from, uint32_t to) {
     if (first <= bin && bin <= last) return;
-    const int from = sh.count[bin] <= (uint32_t)kList ? 0 : bin;
-    if (sh.count[bin] - count_before(from) > (uint32_t)kList) return;  // stays in memory
+    const int b0 = sh.count[bin] <= (uint32_t)kList ? 0 : bin;
+    if (sh.count[bin] - count_before(b0) > (uint32_t)kList) return;  // stays in memory
+    if (b0 == 0) from = 0;
     __syncthreads();
     if (threadIdx.x == 0) sh.listed = 0;
     __syncthreads();
+    const float most = value_of(max(from, key_of(r.top))), least = value_of(to);
     scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
-      if (l != l) l = -INFINITY;
-      const int b = bin_of(r, log2_weight(r, l));
-      if (b < from || b > bin) return;
+      if (!(l <= most && l >= least)) return;
       const uint32_t at = atomicAdd(&sh.listed, 1u);
       if (at >= (uint32_t)kList) return;  // the row changed under the call
       sh.key[at] = key_of(l);
       sh.index[at] = t;
     });
     __syncthreads();
-    first = from;
+    first = b0;
     last = bin;
   }
 
-  // Calls f(key, index, log2 weight) for the bin's tokens, each thread its share.
+  // Calls f(key, index) for the bin's tokens, of keys from..to, each thread its share.
   template <typename F>
-  __device__ __forceinline__ void each(int bin, F f) {
+  __device__ __forceinline__ void each(int bin, uint32_t from, uint32_t to, F f) {
     if (first <= bin && bin <= last) {
       const int n = min((int)sh.listed, kList);
       for (int i = threadIdx.x; i < n; i += kPickThreads) {
-        const double y = log2_weight(r, value_of(sh.key[i]));
-        if (bin_of(r, y) == bin) f(sh.key[i], sh.index[i], y);
+        const uint32_t k = sh.key[i];
+        if (k >= from && k <= to) f(k, sh.index[i]);
       }
     } else {
+      // (the order of the values is that of their keys; NaN is in no range)
+      const float most = value_of(from), least = value_of(to);
       scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
-        if (l != l) l = -INFINITY;
-        const double y = log2_weight(r, l);
-        if (bin_of(r, y) == bin) f(key_of(l), t, y);
+        if (l <= most && l >= least) f(key_of(l), t);
       });
     }
   }
@@ -453,7 +473,7 @@ struct Picker {
   template <typename W>
   __device__ __forceinline__ int differing_bits(W walk, uint32_t* common) {
     uint32_t lo = 0xffffffffu, hi = 0u;
-    walk([&](uint32_t v, double) {
+    walk([&](uint32_t v) {
       lo = min(lo, v);
       hi = max(hi, v);
     });
@@ -464,7 +484,7 @@ struct Picker {
     return bits;
   }
 
-  // The value, among those that `walk` shows with their log2 weights, at which the running
+  // The value, among those that `walk` shows (keys, if weighed), at which the running
   // count or mass exceeds target; before and mass lie ahead of all of them.
   template <typename W>
   __device__ __forceinline__ Found descend(W walk, bool by_count, bool weigh, uint64_t target,
@@ -479,11 +499,11 @@ struct Picker {
       low -= width;
       clear_digits();
       const uint32_t prefix = high == 32 ? 0u : f.key >> high;
-      walk([&](uint32_t v, double y) {
+      walk([&](uint32_t v) {
         if (high < 32 && v >> high != prefix) return;
         const uint32_t d = (v >> low) & ((1u << width) - 1u);
         atomicAdd(&sh.digit_count[d], 1u);
-        const uint64_t w = weigh ? fixed_weight(sh.table, a.shift, y) : 0;
+        const uint64_t w = weigh ? weight(v) : 0;
         if (w) add64(&sh.digit_mass[d], w);
       });
       cross_digit(by_count, target, f.before, f.mass_before);
@@ -498,20 +518,17 @@ struct Picker {
   __device__ __forceinline__ Found find(bool by_count, uint64_t target, int* bin_out) {
     const int bin = crossing(by_count, target);
     *bin_out = bin;
-    list(bin);
+    const uint32_t from = last_key(bin - 1) + 1, to = last_key(bin);
+    list(bin, from, to);
     return descend(
-        [&](auto f) { each(bin, [&](uint32_t k, int, double y) { f(k, y); }); }, by_count, true,
+        [&](auto f) { each(bin, from, to, [&](uint32_t k, int) { f(k); }); }, by_count, true,
         target, count_before(bin), mass_before(bin));
   }
 
   // The index of rank nth (from 0) among the bin's tokens of a key.
   __device__ __forceinline__ int nth_equal(int bin, uint32_t key, uint32_t nth) {
     return (int)descend(
-               [&](auto f) {
-                 each(bin, [&](uint32_t k, int t, double y) {
-                   if (k == key) f((uint32_t)t, y);
-                 });
-               },
+               [&](auto f) { each(bin, key, key, [&](uint32_t, int t) { f((uint32_t)t); }); },
                true, false, nth, 0u, 0u)
         .key;
   }
@@ -580,8 +597,10 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(const SampleArgs a
     bin = bin_of(r, least);
     uint64_t m = 0;
     if (p.mass_before(bin) < kept) {  // else a shorter prefix is there already
-      p.list(bin);
-      p.each(bin, [&](uint32_t, int, double y) {
+      const uint32_t from = p.last_key(bin - 1) + 1, to = p.last_key(bin);
+      p.list(bin, from, to);
+      p.each(bin, from, to, [&](uint32_t key, int) {
+        const double y = log2_weight(r, value_of(key));
         if (y >= least) m += fixed_weight(sh.table, a.shift, y);
       });
       kept = min(kept, p.mass_before(bin) + p.block_sum(m));
