@@ -10,11 +10,13 @@
 // Weights are 64-bit integers (see fixed_weight): sums of them are exact, so LDS and
 // global atomics may add in any order, and workgroups' histograms join without one.
 //
-// Launches: the rows' largest and smallest logits, the histogram (both over many
-// workgroups per row), and one workgroup per row for the positions.  That one reads its
-// row once more: it gathers the tokens from the top through the first range it needs, up
-// to kList of them, in LDS, and most often every position lies among them.  A range that
-// does not fit (thousands of near-equal logits) is walked in memory instead.
+// Launches: the rows' largest and smallest logits, the histogram, the tokens of every
+// range in which one of the positions can lie (all three over many workgroups per row), and
+// one workgroup per row for the positions.  The limits depend on one another (top-p on the
+// weight that top-k leaves, the draw on all of them), but each lies between values that the
+// histogram gives, so the candidates are one to three ranges each, a few hundred tokens;
+// the last workgroup has them in LDS.  Ranges of more than kList tokens (thousands of
+// near-equal logits) stay in memory and are walked there.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -29,10 +31,23 @@ namespace k3 {
 namespace {
 
 constexpr int kBins = 2048;          // of the first histogram
-constexpr int kList = 12288;         // tokens that the last workgroup holds: 96 KB of its LDS
-constexpr int kScanThreads = 256;    // of the passes over a row's parts
+constexpr int kList = 4096;          // candidates of a row that are gathered
+constexpr int kScanThreads = 512;    // of the passes over a row's parts
 constexpr int kPickThreads = 1024;   // of the workgroup that ends a row
 constexpr double kVanish = 64.0;     // weights under 2^-kVanish round to none
+
+constexpr int kRanges = 4;           // top-k's, top-p's, min-p's and the draw's
+constexpr int kSmall = 64;           // tokens that one wave orders
+
+// The ranges of bins in which a row's positions lie, apart and ascending.
+struct RowPlan {
+  int32_t first;                     // lowest index of the largest logit (T not above 0)
+  int32_t ranges;
+  int32_t b0[kRanges], b1[kRanges];  // first and last bin
+  int32_t base[kRanges];             // place of the first in the list, or -1
+  int32_t pad[2];
+};
+static_assert(sizeof(RowPlan) == 64, "one line per row");
 
 struct SampleArgs {
   const void* logits;
@@ -45,6 +60,9 @@ struct SampleArgs {
   uint32_t* ends;      // [rows][parts][2] keys of the parts' largest and smallest logits
   uint32_t* count;     // [rows][kBins]
   uint64_t* mass;      // [rows][kBins]
+  uint32_t* taken;     // [rows][kBins] tokens gathered
+  RowPlan* plan;       // [rows]
+  uint2* list;         // [rows][kList] gathered keys and indices, a range's bins in order
   int rows, vocab, parts, part;  // parts of a row and tokens of one
   int shift;           // weight 1 is 2^shift
 };
@@ -218,7 +236,9 @@ __global__ __launch_bounds__(kScanThreads) void k_sample_ends(const SampleArgs a
   for (int b = part * kScanThreads + threadIdx.x; b < kBins; b += a.parts * kScanThreads) {
     a.count[(uint64_t)row * kBins + b] = 0;
     a.mass[(uint64_t)row * kBins + b] = 0;
+    a.taken[(uint64_t)row * kBins + b] = 0;
   }
+  if (part == 0 && threadIdx.x == 0) a.plan[row].first = a.vocab;
 }
 
 template <typename T>
@@ -258,23 +278,6 @@ __global__ __launch_bounds__(kScanThreads) void k_sample_histogram(const SampleA
   }
 }
 
-struct PickShared {
-  uint32_t count[kBins];  // running counts and masses, each bin's own included
-  uint64_t mass[kBins];
-  double table[64];
-  uint32_t digit_count[256];
-  uint64_t digit_mass[256];
-  uint32_t key[kList];
-  int32_t index[kList];
-  uint32_t listed;
-  uint32_t wave_count[kPickThreads / 64];
-  uint64_t wave_mass[kPickThreads / 64];
-  uint32_t red[2 * kPickThreads / 64];
-  int bin;
-  uint32_t digit, before;
-  uint64_t mass_before;
-};
-
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
   return (uint64_t)__shfl_up((unsigned long long)v, d);
 }
@@ -282,50 +285,30 @@ __device__ __forceinline__ void add64(uint64_t* to, uint64_t v) {
   atomicAdd(reinterpret_cast<unsigned long long*>(to), (unsigned long long)v);
 }
 
-// A position in a row's order: the key of its token and what lies before that key.
-struct Found {
-  uint32_t key;
-  uint32_t before;       // tokens of smaller keys
-  uint64_t mass_before;  // and their weight
-};
+// A row's histogram as running counts and weights, each bin's own included, in the LDS of a
+// workgroup of THREADS.  Every member is called by all of its threads.
+template <int THREADS>
+struct Running {
+  uint32_t count[kBins];
+  uint64_t mass[kBins];
+  uint32_t wave_count[THREADS / 64];
+  uint64_t wave_mass[THREADS / 64];
+  int bin;
 
-// One row's workgroup.  Every member is called by all of its threads.
-template <typename T>
-struct Picker {
-  PickShared& sh;
-  const SampleArgs& a;
-  const T* row;
-  RowParams r;
-  int first = 0, last = -1;  // bins whose tokens are listed
-
-  // The last key of the bins up to `bin`: bins never fall along the keys.  64 keys at a
-  // time; with the two ends of a bin known, tokens are told by their keys alone, without
-  // the fp64 of bin_of (which took half of a pass over the row).
-  __device__ __forceinline__ uint32_t last_key(int bin) const {
-    if (bin < 0) return key_of(r.top) - 1;
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t lo = key_of(r.top), hi = kKeyMasked;  // lo is in, hi is not
-    while (hi - lo > 1) {
-      const uint32_t step = (hi - lo - 1) / 64 + 1;
-      const uint32_t at = lo + (lane + 1) * step;
-      const bool in = at < hi && at > lo && bin_of(r, log2_weight(r, value_of(at))) <= bin;
-      const uint32_t n = (uint32_t)__popcll(__ballot(in));
-      const uint32_t next = lo + (n + 1) * step;
-      lo += n * step;
-      if (n < 64 && next > lo && next < hi) hi = next;
+  __device__ __forceinline__ void load(const SampleArgs& a, int row) {
+    constexpr int kPer = kBins / THREADS;
+    const int b = kPer * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t* gc = a.count + (uint64_t)row * kBins + b;
+    const uint64_t* gm = a.mass + (uint64_t)row * kBins + b;
+    uint32_t cv[kPer], c = 0;
+    uint64_t mv[kPer], m = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      cv[i] = c += gc[i];
+      mv[i] = m += gm[i];
     }
-    return lo;
-  }
-
-  // The histogram, as running sums.
-  __device__ __forceinline__ void load_histogram(int row_index) {
-    const int b = 2 * threadIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t* gc = a.count + (uint64_t)row_index * kBins;
-    const uint64_t* gm = a.mass + (uint64_t)row_index * kBins;
-    const uint32_t c0 = gc[b], c1 = gc[b + 1];
-    const uint64_t m0 = gm[b], m1 = gm[b + 1];
-    uint32_t c = c0 + c1;
-    uint64_t m = m0 + m1;
+    const uint32_t own_c = c;
+    const uint64_t own_m = m;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t cu = __shfl_up(c, d);
@@ -336,93 +319,345 @@ struct Picker {
       }
     }
     if (lane == 63) {
-      sh.wave_count[wave] = c;
-      sh.wave_mass[wave] = m;
+      wave_count[wave] = c;
+      wave_mass[wave] = m;
     }
     __syncthreads();
+    c -= own_c;
+    m -= own_m;
     for (int w = 0; w < wave; ++w) {
-      c += sh.wave_count[w];
-      m += sh.wave_mass[w];
+      c += wave_count[w];
+      m += wave_mass[w];
     }
-    sh.count[b] = c - c1;
-    sh.count[b + 1] = c;
-    sh.mass[b] = m - m1;
-    sh.mass[b + 1] = m;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      count[b + i] = c + cv[i];
+      mass[b + i] = m + mv[i];
+    }
     __syncthreads();
   }
 
-  // The first bin whose running count or mass exceeds target; there is one.
+  __device__ __forceinline__ uint32_t count_before(int b) const { return b ? count[b - 1] : 0u; }
+  __device__ __forceinline__ uint64_t mass_before(int b) const { return b ? mass[b - 1] : 0u; }
+
+  // The first bin whose running count or weight exceeds target; there is one.
   __device__ __forceinline__ int crossing(bool by_count, uint64_t target) {
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int b = 2 * threadIdx.x + i;
-      const uint64_t here = by_count ? sh.count[b] : sh.mass[b];
-      const uint64_t ahead = b == 0 ? 0 : by_count ? sh.count[b - 1] : sh.mass[b - 1];
-      if (ahead <= target && here > target) sh.bin = b;
+    for (int i = 0; i < kBins / THREADS; ++i) {
+      const int b = threadIdx.x + i * THREADS;
+      const uint64_t here = by_count ? count[b] : mass[b];
+      const uint64_t ahead = by_count ? count_before(b) : mass_before(b);
+      if (ahead <= target && here > target) bin = b;
     }
     __syncthreads();
-    return sh.bin;
+    return bin;
   }
+};
 
-  __device__ __forceinline__ uint32_t count_before(int bin) const {
-    return bin ? sh.count[bin - 1] : 0u;
+// The last key of the bins up to `bin`, by a wave: bins never fall along the keys.  64 keys
+// at a time; with the two ends of a range known, its tokens are told by their values,
+// without the fp64 of bin_of (which took half of a pass over the row).
+__device__ __forceinline__ uint32_t last_key(const RowParams& r, int bin) {
+  if (bin < 0) return key_of(r.top) - 1;
+  const uint32_t lane = threadIdx.x & 63;
+  uint32_t lo = key_of(r.top), hi = kKeyMasked;  // lo is in, hi is not
+  while (hi - lo > 1) {
+    const uint32_t step = (hi - lo - 1) / 64 + 1;
+    const uint32_t at = lo + (lane + 1) * step;
+    const bool in = at < hi && at > lo && bin_of(r, log2_weight(r, value_of(at))) <= bin;
+    const uint32_t n = (uint32_t)__popcll(__ballot(in));
+    const uint32_t next = lo + (n + 1) * step;
+    lo += n * step;
+    if (n < 64 && next > lo && next < hi) hi = next;
   }
-  __device__ __forceinline__ uint64_t mass_before(int bin) const {
-    return bin ? sh.mass[bin - 1] : 0u;
-  }
+  return lo;
+}
 
-  // Lists the tokens of the bin (keys up to `to`), with those of every larger logit where
-  // they fit.
-  __device__ __forceinline__ void list(int bin, uint32_t from, uint32_t to) {
-    if (first <= bin && bin <= last) return;
-    const int b0 = sh.count[bin] <= (uint32_t)kList ? 0 : bin;
-    if (sh.count[bin] - count_before(b0) > (uint32_t)kList) return;  // stays in memory
-    if (b0 == 0) from = 0;
-    __syncthreads();
-    if (threadIdx.x == 0) sh.listed = 0;
-    __syncthreads();
-    const float most = value_of(max(from, key_of(r.top))), least = value_of(to);
-    scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
-      if (!(l <= most && l >= least)) return;
-      const uint32_t at = atomicAdd(&sh.listed, 1u);
-      if (at >= (uint32_t)kList) return;  // the row changed under the call
-      sh.key[at] = key_of(l);
-      sh.index[at] = t;
+// A row's limits.
+struct Limits {
+  bool has_k, has_p, has_m;
+  uint64_t k;       // target count of the last of the first top_k
+  double p, least;  // top-p's share, min-p's log2 weight
+  double u;
+};
+
+template <int THREADS>
+__device__ __forceinline__ Limits row_limits(const SampleArgs& a, int row,
+                                             const Running<THREADS>& h) {
+  Limits l;
+  const int k = a.top_k ? a.top_k[row] : 0;
+  // (a first k that ends among the tokens of no weight leaves the sum as it is)
+  l.has_k = k > 0 && k < a.vocab && (uint32_t)k <= h.count[kBins - 2];
+  l.k = (uint64_t)(k - 1);
+  const float p = a.top_p ? a.top_p[row] : 1.f;
+  l.has_p = p < 1.f;
+  l.p = fmax((double)p, 0.0);
+  const float m = a.min_p ? a.min_p[row] : 0.f;
+  l.has_m = m > 0.f;
+  l.least = l.has_m ? log2(fmin((double)m, 1.0)) : 0.0;
+  float u = a.u[row];
+  if (!(u < 1.f)) u = 1.f - 0x1p-24f;
+  l.u = (double)fmaxf(u, 0.f);
+  return l;
+}
+
+// The weight that a top-p prefix has to reach, and the one that the draw has to exceed:
+// both rise with the weight they are shares of.
+__device__ __forceinline__ uint64_t top_p_want(const Limits& l, uint64_t kept) {
+  return max((uint64_t)1, (uint64_t)ceil(l.p * (double)kept));
+}
+__device__ __forceinline__ uint64_t draw_target(const Limits& l, uint64_t kept) {
+  return min((uint64_t)(l.u * (double)kept), kept - 1);
+}
+
+template <typename T>
+__global__ __launch_bounds__(kScanThreads) void k_sample_gather(const SampleArgs a) {
+  const int row = blockIdx.y, part = blockIdx.x;
+  __shared__ Running<kScanThreads> h;
+  __shared__ RowPlan plan;
+  __shared__ uint32_t red[2 * kScanThreads / 64];
+  __shared__ float most[kRanges], least[kRanges];
+  __shared__ uint32_t found, key[kList], index[kList];
+  uint32_t top, bottom;
+  row_ends(a, row, red, kScanThreads, &top, &bottom);
+  if (top == kKeyMasked) return;
+  const RowParams r = row_params(a, row, top, bottom);
+  const T* tokens = static_cast<const T*>(a.logits) + (uint64_t)row * a.vocab;
+  const int t0 = part * a.part, t1 = min(t0 + a.part, a.vocab);
+  if (!r.sampled) {
+    int at = a.vocab;
+    scan(tokens, t0, t1, kScanThreads, [&](float l, int t) {
+      if (l == r.top) at = min(at, t);
     });
-    __syncthreads();
-    first = b0;
-    last = bin;
+    if (at < a.vocab) atomicMin(&a.plan[row].first, at);
+    return;
+  }
+  h.load(a, row);
+  const Limits l = row_limits(a, row, h);
+  // each limit's bins, from what the ones before it leave at least and at most
+  uint64_t lo = h.mass[kBins - 1], hi = lo;
+  int b0[kRanges], b1[kRanges];
+#pragma unroll
+  for (int i = 0; i < kRanges; ++i) {
+    b0[i] = kBins;
+    b1[i] = -1;
+  }
+  if (l.has_k) {
+    b0[0] = b1[0] = h.crossing(true, l.k);
+    lo = h.mass_before(b0[0]);
+    hi = h.mass[b0[0]];
+  }
+  if (l.has_p) {
+    b0[1] = h.crossing(false, top_p_want(l, lo) - 1);
+    b1[1] = h.crossing(false, top_p_want(l, hi) - 1);
+    lo = min(lo, h.mass_before(b0[1]));
+    hi = min(hi, h.mass[b1[1]]);
+  }
+  if (l.has_m) {
+    const int b = bin_of(r, l.least);
+    if (h.mass_before(b) < hi) b0[2] = b1[2] = b;
+    lo = min(lo, h.mass_before(b));
+    hi = min(hi, h.mass[b]);
+  }
+  b0[3] = h.crossing(false, lo ? draw_target(l, lo) : 0);
+  b1[3] = h.crossing(false, draw_target(l, hi));
+  if (threadIdx.x == 0) {
+    // ascending, joined where they meet, and given places while they fit
+    int n = 0, total = 0;
+    int at = -1;
+    for (;;) {
+      int f = kBins, e = -1;  // the next range: the smallest first bin behind `at`
+#pragma unroll
+      for (int i = 0; i < kRanges; ++i)
+        if (b1[i] > at && max(b0[i], at + 1) < f) f = max(b0[i], at + 1);
+      if (f == kBins) break;
+      e = f - 1;
+      for (int again = 0; again < kRanges; ++again)
+#pragma unroll
+        for (int i = 0; i < kRanges; ++i)
+          if (b0[i] <= e + 1 && b1[i] > e && b1[i] >= f) e = b1[i];
+      const int tokens_in = (int)(h.count[e] - h.count_before(f));
+      plan.b0[n] = f;
+      plan.b1[n] = e;
+      plan.base[n] = total + tokens_in <= kList ? total : -1;
+      if (plan.base[n] >= 0) total += tokens_in;
+      ++n;
+      at = e;
+      if (n == kRanges) break;
+    }
+    plan.ranges = n;
+    for (int i = n; i < kRanges; ++i) {
+      plan.b0[i] = kBins;
+      plan.b1[i] = plan.base[i] = -1;
+    }
+    plan.first = a.vocab;
+    found = 0;
+  }
+  __syncthreads();
+  static_assert(kRanges <= kScanThreads / 64, "a wave per range");
+  const int wave = threadIdx.x >> 6;
+  if (wave < kRanges) {
+    const bool any = plan.base[wave] >= 0;
+    const uint32_t from = any ? last_key(r, plan.b0[wave] - 1) + 1 : 0u;
+    const uint32_t to = any ? last_key(r, plan.b1[wave]) : 0u;
+    if ((threadIdx.x & 63) == 0) {
+      most[wave] = any && from <= to ? value_of(from) : -INFINITY;
+      least[wave] = any && from <= to ? value_of(to) : INFINITY;
+    }
+  }
+  if (part == 0 && threadIdx.x < sizeof(RowPlan) / 4)
+    reinterpret_cast<int32_t*>(&a.plan[row])[threadIdx.x] =
+        reinterpret_cast<const int32_t*>(&plan)[threadIdx.x];
+  __syncthreads();
+  float m[kRanges], s[kRanges];
+#pragma unroll
+  for (int i = 0; i < kRanges; ++i) {
+    m[i] = most[i];
+    s[i] = least[i];
+  }
+  scan(tokens, t0, t1, kScanThreads, [&](float v, int t) {
+    bool in = false;
+#pragma unroll
+    for (int i = 0; i < kRanges; ++i) in = in || (v <= m[i] && v >= s[i]);
+    if (!in) return;
+    const uint32_t at = atomicAdd(&found, 1u);
+    if (at >= (uint32_t)kList) return;  // (the row changed under the call)
+    key[at] = key_of(v);
+    index[at] = (uint32_t)t;
+  });
+  __syncthreads();
+  // places by the bins' counters in memory, all at once: one at a time, as tokens were
+  // found, their round trips took most of the launch
+  for (uint32_t i = threadIdx.x; i < min(found, (uint32_t)kList); i += kScanThreads) {
+    const int b = bin_of(r, log2_weight(r, value_of(key[i])));
+    int in = 0;
+    for (int k = 0; k < plan.ranges; ++k)
+      if (plan.b0[k] <= b && b <= plan.b1[k]) in = k;
+    const uint32_t at = plan.base[in] + (h.count_before(b) - h.count_before(plan.b0[in])) +
+                        atomicAdd(&a.taken[(uint64_t)row * kBins + b], 1u);
+    if (at < (uint32_t)kList) a.list[(uint64_t)row * kList + at] = make_uint2(key[i], index[i]);
+  }
+}
+
+struct PickShared {
+  Running<kPickThreads> h;
+  RowPlan plan;
+  double table[64];
+  uint2 list[kList];
+  uint32_t digit_count[256];
+  uint64_t digit_mass[256];
+  uint32_t small_key[kSmall];
+  uint32_t small_index[kSmall];
+  uint64_t small_weight[kSmall];
+  uint32_t small;
+  uint32_t red[2 * kPickThreads / 64];
+  uint64_t wave_mass[kPickThreads / 64];
+  uint32_t digit, before;
+  uint64_t mass;
+  int token;
+};
+
+// A position in a row's order.
+struct Found {
+  uint64_t mass;  // weight through its token
+  int token;      // if asked for
+};
+
+// One row's workgroup.  Every member is called by all of its threads.
+template <typename T>
+struct Picker {
+  PickShared& sh;
+  const SampleArgs& a;
+  const T* row;
+  RowParams r;
+
+  __device__ __forceinline__ uint64_t weight(uint32_t key) const {
+    return fixed_weight(sh.table, a.shift, log2_weight(r, value_of(key)));
   }
 
-  // Calls f(key, index) for the bin's tokens, of keys from..to, each thread its share.
-  template <typename F>
-  __device__ __forceinline__ void each(int bin, uint32_t from, uint32_t to, F f) {
-    if (first <= bin && bin <= last) {
-      const int n = min((int)sh.listed, kList);
-      for (int i = threadIdx.x; i < n; i += kPickThreads) {
-        const uint32_t k = sh.key[i];
-        if (k >= from && k <= to) f(k, sh.index[i]);
+  // Where a bin's tokens are: a part of the list, or a range of values in memory.
+  struct Place {
+    int at, n;         // n < 0: in memory
+    float most, least;
+  };
+  __device__ __forceinline__ Place place(int bin) const {
+    Place p{0, -1, 0.f, 0.f};
+    for (int i = 0; i < sh.plan.ranges; ++i)
+      if (sh.plan.b0[i] <= bin && bin <= sh.plan.b1[i] && sh.plan.base[i] >= 0) {
+        const uint32_t before = sh.h.count_before(bin);
+        p.at = sh.plan.base[i] + (int)(before - sh.h.count_before(sh.plan.b0[i]));
+        p.n = (int)(sh.h.count[bin] - before);
+        p.n = min(p.n, kList - p.at);
       }
+    if (p.n < 0) {
+      p.most = value_of(last_key(r, bin - 1) + 1);
+      p.least = value_of(last_key(r, bin));
+    }
+    return p;
+  }
+
+  // Calls f(key, index) for the tokens of a bin, each thread its share.
+  template <typename F>
+  __device__ __forceinline__ void each(const Place& p, F f) {
+    if (p.n >= 0) {
+      for (int i = threadIdx.x; i < p.n; i += kPickThreads) f(sh.list[p.at + i].x, sh.list[p.at + i].y);
     } else {
-      // (the order of the values is that of their keys; NaN is in no range)
-      const float most = value_of(from), least = value_of(to);
       scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
-        if (l <= most && l >= least) f(key_of(l), t);
+        if (l <= p.most && l >= p.least) f(key_of(l), (uint32_t)t);
       });
     }
   }
 
-  // Of the 256 digits, the first at which the running count or mass (what lies before the
-  // digits included) exceeds target: into sh.digit, sh.before and sh.mass_before.
-  __device__ __forceinline__ void cross_digit(bool by_count, uint64_t target, uint32_t before,
-                                              uint64_t mass) {
+  // What lies before a set of values, what the set holds, and the bits all of them share.
+  struct Part {
+    uint32_t before, n;
+    uint64_t mass;    // weight before it
+    uint32_t prefix;  // the values' bits from `low` up, in place
+    int low;
+  };
+
+  // Narrows the part to the bits in which its values differ.  walk(f) calls f(value).
+  template <typename W>
+  __device__ __forceinline__ void narrow(W walk, Part* part) {
+    uint32_t lo = 0xffffffffu, hi = 0u;
+    walk([&](uint32_t v) {
+      lo = min(lo, v);
+      hi = max(hi, v);
+    });
+    block_ends(sh.red, kPickThreads / 64, &lo, &hi);
+    const uint32_t x = lo ^ hi;
+    part->low = x ? 32 - __clz((int)x) : 0;
+    part->prefix = part->low == 32 ? 0u : lo >> part->low << part->low;
+  }
+
+  __device__ __forceinline__ bool in(const Part& part, uint32_t v) const {
+    return part.low == 32 || v >> part.low == part.prefix >> part.low;
+  }
+
+  // Narrows the part by its next (up to) eight bits, to the values at which the running
+  // count or weight exceeds target.
+  template <typename W>
+  __device__ __forceinline__ void digit(W walk, bool by_count, bool weigh, uint64_t target,
+                                        Part* part) {
+    const int width = min(part->low, 8), low = part->low - width;
+    __syncthreads();
+    if (threadIdx.x < 256) {
+      sh.digit_count[threadIdx.x] = 0;
+      sh.digit_mass[threadIdx.x] = 0;
+    }
+    __syncthreads();
+    walk([&](uint32_t v) {
+      if (!in(*part, v)) return;
+      const uint32_t d = (v >> low) & ((1u << width) - 1u);
+      atomicAdd(&sh.digit_count[d], 1u);
+      const uint64_t w = weigh ? weight(v) : 0;
+      if (w) add64(&sh.digit_mass[d], w);
+    });
     __syncthreads();
     if (threadIdx.x < 64) {
-      uint32_t c[4];
-      uint64_t m[4];
-      uint32_t cs = 0;
-      uint64_t ms = 0;
+      uint32_t c[4], cs = 0;
+      uint64_t m[4], ms = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         c[i] = sh.digit_count[4 * threadIdx.x + i];
@@ -441,8 +676,8 @@ struct Picker {
           mi += mu;
         }
       }
-      uint32_t cr = before + ci - cs;
-      uint64_t mr = mass + mi - ms;
+      uint32_t cr = part->before + ci - cs;
+      uint64_t mr = part->mass + mi - ms;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const uint64_t ahead = by_count ? cr : mr;
@@ -450,91 +685,85 @@ struct Picker {
         if (ahead <= target && here > target) {
           sh.digit = 4 * threadIdx.x + i;
           sh.before = cr;
-          sh.mass_before = mr;
+          sh.mass = mr;
         }
         cr += c[i];
         mr += m[i];
       }
     }
     __syncthreads();
+    part->low = low;
+    part->prefix |= sh.digit << low;
+    part->before = sh.before;
+    part->mass = sh.mass;
+    part->n = sh.digit_count[sh.digit & 255u];
   }
 
-  __device__ __forceinline__ void clear_digits() {
-    __syncthreads();
-    if (threadIdx.x < 256) {
-      sh.digit_count[threadIdx.x] = 0;
-      sh.digit_mass[threadIdx.x] = 0;
-    }
-    __syncthreads();
-  }
-
-  // The bits in which the values that `walk` shows differ, from the highest differing one
-  // down; their common part goes to *common.
-  template <typename W>
-  __device__ __forceinline__ int differing_bits(W walk, uint32_t* common) {
-    uint32_t lo = 0xffffffffu, hi = 0u;
-    walk([&](uint32_t v) {
-      lo = min(lo, v);
-      hi = max(hi, v);
-    });
-    block_ends(sh.red, kPickThreads / 64, &lo, &hi);
-    const uint32_t x = lo ^ hi;
-    const int bits = x ? 32 - __clz((int)x) : 0;
-    *common = bits == 32 ? 0u : lo >> bits << bits;
-    return bits;
-  }
-
-  // The value, among those that `walk` shows (keys, if weighed), at which the running
-  // count or mass exceeds target; before and mass lie ahead of all of them.
-  template <typename W>
-  __device__ __forceinline__ Found descend(W walk, bool by_count, bool weigh, uint64_t target,
-                                           uint32_t before, uint64_t mass) {
-    Found f;
-    int low = differing_bits(walk, &f.key);
-    f.before = before;
-    f.mass_before = mass;
-    while (low > 0) {
-      const int width = min(low, 8);
-      const int high = low;
-      low -= width;
-      clear_digits();
-      const uint32_t prefix = high == 32 ? 0u : f.key >> high;
-      walk([&](uint32_t v) {
-        if (high < 32 && v >> high != prefix) return;
-        const uint32_t d = (v >> low) & ((1u << width) - 1u);
-        atomicAdd(&sh.digit_count[d], 1u);
-        const uint64_t w = weigh ? weight(v) : 0;
-        if (w) add64(&sh.digit_mass[d], w);
+  // The first token at which the row's running count or weight exceeds target.
+  __device__ __forceinline__ Found find(bool by_count, uint64_t target, bool ask_token) {
+    const int bin = sh.h.crossing(by_count, target);
+    const Place at = place(bin);
+    auto keys = [&](auto f) { each(at, [&](uint32_t k, uint32_t) { f(k); }); };
+    Part part;
+    part.before = sh.h.count_before(bin);
+    part.mass = sh.h.mass_before(bin);
+    part.n = sh.h.count[bin] - part.before;
+    part.prefix = 0;
+    part.low = 32;
+    if (part.n > kSmall) narrow(keys, &part);
+    while (part.n > kSmall && part.low > 0) digit(keys, by_count, true, target, &part);
+    if (part.n <= kSmall) {
+      // few tokens: one wave ranks each against all of them, by key and index
+      __syncthreads();
+      if (threadIdx.x == 0) sh.small = 0;
+      __syncthreads();
+      each(at, [&](uint32_t k, uint32_t t) {
+        if (!in(part, k)) return;
+        const uint32_t i = atomicAdd(&sh.small, 1u);
+        if (i >= (uint32_t)kSmall) return;  // (the row changed under the call)
+        sh.small_key[i] = k;
+        sh.small_index[i] = t;
+        sh.small_weight[i] = weight(k);
       });
-      cross_digit(by_count, target, f.before, f.mass_before);
-      f.key |= sh.digit << low;
-      f.before = sh.before;
-      f.mass_before = sh.mass_before;
+      __syncthreads();
+      if (threadIdx.x < 64) {
+        const int n = min((int)sh.small, kSmall), i = max(min((int)threadIdx.x, n - 1), 0);
+        const uint32_t k = sh.small_key[i], t = sh.small_index[i];
+        const uint64_t w = sh.small_weight[i];
+        uint64_t c = part.before, m = part.mass;
+        for (int j = 0; j < n; ++j) {
+          const uint32_t kj = sh.small_key[j];
+          if (kj < k || (kj == k && sh.small_index[j] < t)) {
+            ++c;
+            m += sh.small_weight[j];
+          }
+        }
+        const uint64_t ahead = by_count ? c : m, here = by_count ? c + 1 : m + w;
+        if ((int)threadIdx.x < n && ahead <= target && here > target) {
+          sh.mass = m + w;
+          sh.token = (int)t;
+        }
+      }
+      __syncthreads();
+      return Found{sh.mass, sh.token};
+    }
+    // many tokens of one key: whole weights of it, in the order of their indices
+    const uint32_t key = part.prefix;
+    const uint64_t w = weight(key);
+    const uint64_t nth = by_count ? target - part.before : (target - part.mass) / w;
+    Found f{part.mass + (nth + 1) * w, -1};
+    if (ask_token) {
+      auto indices = [&](auto g) {
+        each(at, [&](uint32_t k, uint32_t t) {
+          if (k == key) g(t);
+        });
+      };
+      Part p{0u, part.n, 0u, 0u, 32};
+      narrow(indices, &p);
+      while (p.low > 0) digit(indices, true, false, nth, &p);
+      f.token = (int)p.prefix;
     }
     return f;
-  }
-
-  // The first token at which the row's running count or mass exceeds target.
-  __device__ __forceinline__ Found find(bool by_count, uint64_t target, int* bin_out) {
-    const int bin = crossing(by_count, target);
-    *bin_out = bin;
-    const uint32_t from = last_key(bin - 1) + 1, to = last_key(bin);
-    list(bin, from, to);
-    return descend(
-        [&](auto f) { each(bin, from, to, [&](uint32_t k, int) { f(k); }); }, by_count, true,
-        target, count_before(bin), mass_before(bin));
-  }
-
-  // The index of rank nth (from 0) among the bin's tokens of a key.
-  __device__ __forceinline__ int nth_equal(int bin, uint32_t key, uint32_t nth) {
-    return (int)descend(
-               [&](auto f) { each(bin, key, key, [&](uint32_t, int t) { f((uint32_t)t); }); },
-               true, false, nth, 0u, 0u)
-        .key;
-  }
-
-  __device__ __forceinline__ uint64_t weight(uint32_t key) const {
-    return fixed_weight(sh.table, a.shift, log2_weight(r, value_of(key)));
   }
 
   __device__ __forceinline__ uint64_t block_sum(uint64_t m) {
@@ -561,58 +790,40 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(const SampleArgs a
     return;
   }
   const RowParams r = row_params(a, ri, top, bottom);
-  if (!r.sampled) {  // the lowest index of the largest logit
-    int at = a.vocab;
-    scan(row, 0, a.vocab, kPickThreads, [&](float l, int t) {
-      if (l == r.top) at = min(at, t);
-    });
-    uint32_t lo = (uint32_t)at, hi = 0u;
-    block_ends(sh.red, kPickThreads / 64, &lo, &hi);
-    if (threadIdx.x == 0) a.tokens[ri] = (int)lo;
+  if (!r.sampled) {
+    if (threadIdx.x == 0) a.tokens[ri] = a.plan[ri].first;
     return;
   }
   fill_table(sh.table);
+  if (threadIdx.x < sizeof(RowPlan) / 4)
+    reinterpret_cast<int32_t*>(&sh.plan)[threadIdx.x] =
+        reinterpret_cast<const int32_t*>(&a.plan[ri])[threadIdx.x];
+  sh.h.load(a, ri);
+  int listed = 0;
+  for (int i = 0; i < sh.plan.ranges; ++i)
+    if (sh.plan.base[i] >= 0)
+      listed = sh.plan.base[i] +
+               (int)(sh.h.count[sh.plan.b1[i]] - sh.h.count_before(sh.plan.b0[i]));
+  for (int i = threadIdx.x; i < min(listed, kList); i += kPickThreads)
+    sh.list[i] = a.list[(uint64_t)ri * kList + i];
   Picker<T> p{sh, a, row, r};
-  p.load_histogram(ri);
-  int bin;
-  uint64_t kept = sh.mass[kBins - 1];  // weight of the shortest prefix so far
-  const int k = a.top_k ? a.top_k[ri] : 0;
-  // (a first k that ends among the tokens of no weight leaves the sum as it is)
-  if (k > 0 && k < a.vocab && (uint32_t)k <= sh.count[kBins - 2]) {
-    const Found f = p.find(true, (uint64_t)(k - 1), &bin);
-    kept = f.mass_before + (uint64_t)((uint32_t)k - f.before) * p.weight(f.key);
-  }
-  const float top_p = a.top_p ? a.top_p[ri] : 1.f;
-  if (top_p < 1.f) {
-    // the first prefix with a sum of at least top_p times the top-k one's
-    const uint64_t want =
-        max((uint64_t)1, (uint64_t)ceil(fmax((double)top_p, 0.0) * (double)kept));
-    const Found f = p.find(false, want - 1, &bin);
-    const uint64_t w = p.weight(f.key);
-    kept = min(kept, f.mass_before + (want - f.mass_before + w - 1) / w * w);
-  }
-  const float min_p = a.min_p ? a.min_p[ri] : 0.f;
-  if (min_p > 0.f) {
-    const double least = log2(fmin((double)min_p, 1.0));
-    bin = bin_of(r, least);
-    uint64_t m = 0;
-    if (p.mass_before(bin) < kept) {  // else a shorter prefix is there already
-      const uint32_t from = p.last_key(bin - 1) + 1, to = p.last_key(bin);
-      p.list(bin, from, to);
-      p.each(bin, from, to, [&](uint32_t key, int) {
+  const Limits l = row_limits(a, ri, sh.h);
+  uint64_t kept = sh.h.mass[kBins - 1];  // weight of the shortest prefix so far
+  if (l.has_k) kept = p.find(true, l.k, false).mass;
+  if (l.has_p) kept = min(kept, p.find(false, top_p_want(l, kept) - 1, false).mass);
+  if (l.has_m) {
+    const int bin = bin_of(r, l.least);
+    if (sh.h.mass_before(bin) < kept) {  // else a shorter prefix is there already
+      uint64_t m = 0;
+      __syncthreads();
+      p.each(p.place(bin), [&](uint32_t key, uint32_t) {
         const double y = log2_weight(r, value_of(key));
-        if (y >= least) m += fixed_weight(sh.table, a.shift, y);
+        if (y >= l.least) m += fixed_weight(sh.table, a.shift, y);
       });
-      kept = min(kept, p.mass_before(bin) + p.block_sum(m));
+      kept = min(kept, sh.h.mass_before(bin) + p.block_sum(m));
     }
   }
-  float u = a.u[ri];
-  if (!(u < 1.f)) u = 1.f - 0x1p-24f;
-  u = fmaxf(u, 0.f);
-  const uint64_t target = min((uint64_t)((double)u * (double)kept), kept - 1);
-  const Found f = p.find(false, target, &bin);
-  const uint32_t nth = (uint32_t)((target - f.mass_before) / p.weight(f.key));
-  const int t = p.nth_equal(bin, f.key, nth);
+  const int t = p.find(false, draw_target(l, kept), true).token;
   if (threadIdx.x == 0) a.tokens[ri] = t;
 }
 
@@ -620,7 +831,7 @@ uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
 
 struct SampleLayout {
   int parts, part;
-  uint64_t count, mass, bytes;  // offsets of the histograms behind the parts' ends
+  uint64_t count, mass, taken, plan, list, bytes;  // offsets behind the parts' ends
   SampleLayout(int rows, int vocab) {
     // parts of at least 4096 tokens, about two workgroups per CU over all rows
     const int want = std::max(1, 512 / rows);
@@ -629,7 +840,10 @@ struct SampleLayout {
     parts = (vocab + part - 1) / part;
     count = align256(8ull * rows * parts);
     mass = count + align256(4ull * rows * kBins);
-    bytes = mass + align256(8ull * rows * kBins);
+    taken = mass + align256(8ull * rows * kBins);
+    plan = taken + align256(4ull * rows * kBins);
+    list = plan + align256(sizeof(RowPlan) * (uint64_t)rows);
+    bytes = list + align256(sizeof(uint2) * (uint64_t)rows * kList);
   }
 };
 
@@ -668,12 +882,14 @@ int sample_check(const K3HipSampleV1* op, bool sizes) {
 template <typename T>
 int sample_launch(const SampleArgs& a, hipStream_t st) {
   const dim3 grid((unsigned)a.parts, (unsigned)a.rows);
-  for (int step = 0; step < 3; ++step) {
+  for (int step = 0; step < 4; ++step) {
     TimedLaunch tl(KC_ROUTE, st);
     if (step == 0)
       launch_timed(tl, k_sample_ends<T>, grid, dim3(kScanThreads), 0, st, a);
     else if (step == 1)
       launch_timed(tl, k_sample_histogram<T>, grid, dim3(kScanThreads), 0, st, a);
+    else if (step == 2)
+      launch_timed(tl, k_sample_gather<T>, grid, dim3(kScanThreads), 0, st, a);
     else
       launch_timed(tl, k_sample_pick<T>, dim3((unsigned)a.rows), dim3(kPickThreads), 0, st, a);
     const hipError_t e = hipGetLastError();
@@ -723,6 +939,9 @@ int k3_hip_sample(const K3HipSampleV1* op, void* workspace, uint64_t workspace_b
   a.ends = reinterpret_cast<uint32_t*>(ws);
   a.count = reinterpret_cast<uint32_t*>(ws + l.count);
   a.mass = reinterpret_cast<uint64_t*>(ws + l.mass);
+  a.taken = reinterpret_cast<uint32_t*>(ws + l.taken);
+  a.plan = reinterpret_cast<RowPlan*>(ws + l.plan);
+  a.list = reinterpret_cast<uint2*>(ws + l.list);
   a.rows = (int)op->rows;
   a.vocab = (int)op->vocabulary;
   a.parts = l.parts;
