@@ -219,23 +219,65 @@ __device__ __forceinline__ void terms3(float v, uint32_t (&t)[3]) {
   t[2] = nearest_bf16(r - __uint_as_float(t[1] << 16));
 }
 
-// fp32 rows to three planes [3][rows][pitch / 2] (pitch in bytes, zeros past cols); with
-// xs, scaled by the power of two that brings the row's largest finite value into
-// [1, 2), whose inverse goes to xs[row].
+// The two nearest BF16 values, by the hardware's convert: finite ones that round past the
+// largest become infinite, so only for values scaled into [-2, 2].
+__device__ __forceinline__ float head_of(uint32_t pair, int i) {
+  return __uint_as_float(i ? pair & 0xffff0000u : pair << 16);
+}
+
+// fp32 rows to three planes [3][rows_out][pitch / 2] (pitch in bytes, zeros past cols and in
+// rows past `rows`); with xs, scaled by the power of two that brings the row's largest
+// finite value into [1, 2), whose inverse goes to xs[row].  A thread takes eight
+// neighbouring values at a time, kHeld such groups of a row in registers between the
+// search for the largest and the split (rows of up to 8192 values are read once).
+constexpr int kHeld = 4;
+template <bool kScaled>
 __global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x,
                                                     uint8_t* __restrict__ planes,
                                                     float* __restrict__ xs, int rows, int cols,
-                                                    uint32_t pitch) {
-  const uint64_t plane = (uint64_t)rows * pitch;
+                                                    int rows_out, uint32_t pitch, int aligned) {
+  const uint64_t plane = (uint64_t)rows_out * pitch;
   __shared__ float red[4];
-  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+  const int groups = (int)(pitch / 16);
+  for (int row = blockIdx.x; row < rows_out; row += gridDim.x) {
     const float* p = x + (uint64_t)row * cols;
+    auto load = [&](int g, float (&v)[8]) {
+      const int c = 8 * g;
+      if (row < rows && aligned && c + 8 <= cols) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 q = *reinterpret_cast<const f32x4*>(p + c + 4 * h);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[4 * h + i] = q[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = row < rows && c + i < cols ? p[c + i] : 0.f;
+      }
+    };
+    float held[kHeld][8];
     float scale = 1.f;
-    if (xs) {
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int g = threadIdx.x + 256 * k;
+      if (g < groups) load(g, held[k]);
+    }
+    if constexpr (kScaled) {
       float most = 0.f;
-      for (int c = threadIdx.x; c < cols; c += 256) {
-        const float a = fabsf(p[c]);
-        if (a < INFINITY) most = fmaxf(most, a);
+      auto see = [&](const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float a = fabsf(v[i]);
+          most = a < INFINITY ? fmaxf(most, a) : most;
+        }
+      };
+#pragma unroll
+      for (int k = 0; k < kHeld; ++k)
+        if ((int)threadIdx.x + 256 * k < groups) see(held[k]);
+      for (int g = threadIdx.x + 256 * kHeld; g < groups; g += 256) {
+        float v[8];
+        load(g, v);
+        see(v);
       }
 #pragma unroll
       for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
@@ -246,29 +288,60 @@ __global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x,
       // exponents -126 .. 126, so that the scale and its inverse are normal numbers
       const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
       if (most > 0.f) scale = __uint_as_float((uint32_t)(127 - e) << 23);
-      if (threadIdx.x == 0) xs[row] = most > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+      if (threadIdx.x == 0 && row < rows)
+        xs[row] = most > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
     }
-    uint32_t* d = reinterpret_cast<uint32_t*>(planes + (uint64_t)row * pitch);
-    for (int c = 2 * threadIdx.x; c < (int)(pitch / 2); c += 512) {
-      uint32_t lo[3], hi[3];
-      terms3(c < cols ? p[c] * scale : 0.f, lo);
-      terms3(c + 1 < cols ? p[c + 1] * scale : 0.f, hi);
+    uint8_t* d = planes + (uint64_t)row * pitch;
+    auto split = [&](int g, const float (&v)[8]) {
+      u32x4 t[3];
 #pragma unroll
-      for (int i = 0; i < 3; ++i) d[i * (plane / 4) + c / 2] = lo[i] | hi[i] << 16;
+      for (int q = 0; q < 4; ++q) {
+        const float a = v[2 * q] * scale, b = v[2 * q + 1] * scale;
+        if constexpr (kScaled) {
+          const uint32_t t0 = bf16_pair(a, b);
+          // an infinity or NaN is its first term alone
+          const float ra = fabsf(a) < INFINITY ? a - head_of(t0, 0) : 0.f;
+          const float rb = fabsf(b) < INFINITY ? b - head_of(t0, 1) : 0.f;
+          const uint32_t t1 = bf16_pair(ra, rb);
+          t[0][q] = t0;
+          t[1][q] = t1;
+          t[2][q] = bf16_pair(ra - head_of(t1, 0), rb - head_of(t1, 1));
+        } else {
+          uint32_t lo[3], hi[3];
+          terms3(a, lo);
+          terms3(b, hi);
+#pragma unroll
+          for (int i = 0; i < 3; ++i) t[i][q] = lo[i] | hi[i] << 16;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4*>(d + i * plane + 16ull * g) = t[i];
+    };
+#pragma unroll
+    for (int k = 0; k < kHeld; ++k) {
+      const int g = threadIdx.x + 256 * k;
+      if (g < groups) split(g, held[k]);
+    }
+    for (int g = threadIdx.x + 256 * kHeld; g < groups; g += 256) {
+      float v[8];
+      load(g, v);
+      split(g, v);
     }
   }
 }
 
-// Rows of `bytes` bytes to rows of `pitch` (a multiple of 16), zeros behind.
+// Rows to rows of `pitch` bytes (a multiple of 16), zeros behind each and in the rows from
+// `rows` to rows_out.
 template <typename T>
 __global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u32x4* __restrict__ dst,
-                                                   int rows, int cols, uint32_t pitch) {
+                                                   int rows, int cols, int rows_out,
+                                                   uint32_t pitch) {
   constexpr int kPer = 16 / (int)sizeof(T);
   const uint32_t chunks = pitch / 16;
-  const uint64_t total = (uint64_t)rows * chunks;
+  const uint64_t total = (uint64_t)rows_out * chunks;
   for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
     const uint64_t row = t / chunks;
-    const int c0 = (int)(t - row * chunks) * kPer;
+    const int c0 = row < (uint64_t)rows ? (int)(t - row * chunks) * kPer : cols;
     const T* p = src + row * cols;
     u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
@@ -281,43 +354,83 @@ __global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u3
 }
 
 // dg = grad f_g(g, u) and du = grad f_u(g, u) of [rows][cols] values as BF16 planes
-// [terms][rows][2 half]: dg at columns [0, cols), du at [half, half + cols), zeros in the
+// [terms][rows_out][2 half]: dg at columns [0, cols), du at [half, half + cols), zeros in the
 // rest; half is a multiple of 8.  One term rounds to BF16, three keep all 24 bits.
 __device__ __forceinline__ float widen(uint16_t b) { return bf16_bits_to_f32(b); }
 __device__ __forceinline__ float widen(float f) { return f; }
 
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, bool vec, int n, float (&v)[8]) {
+  if (vec && n >= 8) {
+    constexpr int kPer = 16 / (int)sizeof(T);
+#pragma unroll
+    for (int h = 0; h < 8 / kPer; ++h) {
+      const u32x4 q = *reinterpret_cast<const u32x4*>(p + kPer * h);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i)
+        v[kPer * h + i] = sizeof(T) == 4 ? __uint_as_float(q[i % 4])
+                                         : head_of(q[i / 2 % 4], i % 2);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? widen(p[i]) : 0.f;
+  }
+}
+
+// Eight neighbouring columns per thread.
 template <typename T, int TERMS>
 __global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, const T* __restrict__ u,
                                                     const T* __restrict__ grad,
                                                     uint16_t* __restrict__ planes, int rows,
-                                                    int cols, int half, int act) {
-  const uint64_t plane = (uint64_t)rows * 2 * half;
-  const uint64_t total = (uint64_t)rows * half;
+                                                    int cols, int rows_out, int half, int act,
+                                                    int vec) {
+  const uint64_t plane = (uint64_t)rows_out * 2 * half;
+  const uint32_t groups = (uint32_t)half / 8;
+  const uint64_t total = (uint64_t)rows_out * groups;
   for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
-    const uint64_t row = t / (uint32_t)half;
-    const int c = (int)(t - row * (uint32_t)half);
-    float dg = 0.f, du = 0.f;
-    if (c < cols) {
-      const uint64_t at = row * cols + c;
-      const float gv = widen(g[at]), uv = widen(u[at]), d = widen(grad[at]);
-      const float sig = 1.0f / (1.0f + expf(-gv));
-      if (act == K3_ACT_SILU) {
-        dg = d * uv * (sig * (1.0f + gv * (1.0f - sig)));
-        du = d * (gv * sig);
+    const uint64_t row = t / groups;
+    const int c = 8 * (int)(t - row * groups);
+    const int n = row < (uint64_t)rows ? cols - c : 0;
+    const uint64_t at = row * cols + c;
+    float gv[8], uv[8], dv[8];
+    load8(g + at, vec, n, gv);
+    load8(u + at, vec, n, uv);
+    load8(grad + at, vec, n, dv);
+    u32x4 og[TERMS], ou[TERMS];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float dg = 0.f, du = 0.f;
+      if (i < n) {
+        const float sig = 1.0f / (1.0f + expf(-gv[i]));
+        if (act == K3_ACT_SILU) {
+          dg = dv[i] * uv[i] * (sig * (1.0f + gv[i] * (1.0f - sig)));
+          du = dv[i] * (gv[i] * sig);
+        } else {
+          const float a = tanhf(gv[i] / 4.0f), b = tanhf(uv[i] / 25.0f);
+          dg = dv[i] * (25.0f * b) * ((1.0f - a * a) * sig + 4.0f * a * (sig * (1.0f - sig)));
+          du = dv[i] * (4.0f * a * sig) * (1.0f - b * b);
+        }
+      }
+      uint32_t tg[3], tu[3];
+      if constexpr (TERMS == 1) {
+        const uint32_t both = bf16_pair(dg, du);
+        tg[0] = both & 0xffffu;
+        tu[0] = both >> 16;
       } else {
-        const float a = tanhf(gv / 4.0f), b = tanhf(uv / 25.0f);
-        dg = d * (25.0f * b) * ((1.0f - a * a) * sig + 4.0f * a * (sig * (1.0f - sig)));
-        du = d * (4.0f * a * sig) * (1.0f - b * b);
+        terms3(dg, tg);
+        terms3(du, tu);
+      }
+#pragma unroll
+      for (int k = 0; k < TERMS; ++k) {
+        og[k][i / 2] = i % 2 ? og[k][i / 2] | tg[k] << 16 : tg[k];
+        ou[k][i / 2] = i % 2 ? ou[k][i / 2] | tu[k] << 16 : tu[k];
       }
     }
     uint16_t* o = planes + row * 2 * half + c;
-    uint32_t tg[3], tu[3];
-    terms3(dg, tg);
-    terms3(du, tu);
 #pragma unroll
-    for (int i = 0; i < TERMS; ++i) {
-      o[i * plane] = (uint16_t)tg[i];
-      o[i * plane + half] = (uint16_t)tu[i];
+    for (int k = 0; k < TERMS; ++k) {
+      *reinterpret_cast<u32x4*>(o + k * plane) = og[k];
+      *reinterpret_cast<u32x4*>(o + k * plane + half) = ou[k];
     }
   }
 }
@@ -350,44 +463,58 @@ int launched_or(TimedLaunch& tl, const char* what) {
   return spine_fail(K3_SPINE_E_RUNTIME, "%s: %s", what, hipGetErrorString(err));
 }
 
-int pack_rows(const void* src, void* dst, int elem, int rows, int cols, uint32_t pitch,
-              hipStream_t st) {
+int pack_rows(const void* src, void* dst, int elem, int rows, int cols, int rows_out,
+              uint32_t pitch, hipStream_t st) {
   TimedLaunch tl(KC_SPLIT, st);
-  const unsigned grid = grid_for((uint64_t)rows * (pitch / 16));
+  const unsigned grid = grid_for((uint64_t)rows_out * (pitch / 16));
   if (elem == 2)
     launch_timed(tl, k_pack_rows<uint16_t>, dim3(grid), dim3(256), 0, st,
-                 static_cast<const uint16_t*>(src), static_cast<u32x4*>(dst), rows, cols, pitch);
+                 static_cast<const uint16_t*>(src), static_cast<u32x4*>(dst), rows, cols, rows_out,
+                 pitch);
   else
     launch_timed(tl, k_pack_rows<uint8_t>, dim3(grid), dim3(256), 0, st,
-                 static_cast<const uint8_t*>(src), static_cast<u32x4*>(dst), rows, cols, pitch);
+                 static_cast<const uint8_t*>(src), static_cast<u32x4*>(dst), rows, cols, rows_out,
+                 pitch);
   return launched_or(tl, "dense operand layout");
 }
 
-int split_rows(const void* x, void* planes, float* xs, int rows, int cols, uint32_t pitch,
-               hipStream_t st) {
+int split_rows(const void* x, void* planes, float* xs, int rows, int cols, int rows_out,
+               uint32_t pitch, hipStream_t st) {
   TimedLaunch tl(KC_SPLIT, st);
-  launch_timed(tl, k_split_rows, dim3((unsigned)std::min(rows, 1 << 16)), dim3(256), 0, st,
-               static_cast<const float*>(x), static_cast<uint8_t*>(planes), xs, rows, cols, pitch);
+  const dim3 grid((unsigned)std::min(rows_out, 1 << 16));
+  const int aligned = cols % 4 == 0 && aligned16(x);
+  if (xs)
+    launch_timed(tl, k_split_rows<true>, grid, dim3(256), 0, st, static_cast<const float*>(x),
+                 static_cast<uint8_t*>(planes), xs, rows, cols, rows_out, pitch, aligned);
+  else
+    launch_timed(tl, k_split_rows<false>, grid, dim3(256), 0, st, static_cast<const float*>(x),
+                 static_cast<uint8_t*>(planes), xs, rows, cols, rows_out, pitch, aligned);
   return launched_or(tl, "dense activation terms");
 }
+
+// Operands that are laid out anew get a K of whole steps where K runs over their rows
+// (`along`), zeros in the added ones: the rest of K that is no whole step is the slow part
+// of a product.
 
 // A matrix as an operand: in place where its rows are whole 16-byte pieces, else a
 // copy of it with rows that are.
 struct Matrix {
   const void* src;
-  int elem, rows, cols;
+  int elem, rows, cols, rows_out;
   uint32_t pitch;
   uint8_t* copy = nullptr;  // scratch of the copy
   bool copied;
-  Matrix(const void* p, int elem_, int rows_, int cols_, Scratch& s)
-      : src(p), elem(elem_), rows(rows_), cols(cols_) {
+  Matrix(const void* p, int elem_, int rows_, int cols_, bool along, Scratch& s)
+      : src(p), elem(elem_), rows(rows_), cols(cols_), rows_out(rows_) {
     pitch = round_up((uint32_t)cols * elem, 16);
     copied = pitch != (uint32_t)cols * elem || !aligned16(p);
-    if (copied) copy = s.take((uint64_t)rows * pitch);
+    if (!copied) return;
+    if (along) rows_out = (int)round_up((uint32_t)rows, kStep);
+    copy = s.take((uint64_t)rows_out * pitch);
   }
   const uint8_t* data() const { return copied ? copy : static_cast<const uint8_t*>(src); }
   int fill(hipStream_t st) const {
-    return copied ? pack_rows(src, copy, elem, rows, cols, pitch, st) : K3_SPINE_OK;
+    return copied ? pack_rows(src, copy, elem, rows, cols, rows_out, pitch, st) : K3_SPINE_OK;
   }
 };
 
@@ -395,64 +522,76 @@ struct Matrix {
 struct Activation {
   const void* src;
   bool f32;
-  int rows, cols;
+  int rows, cols, rows_out;
   uint32_t pitch;
   uint8_t* planes = nullptr;
   float* xs = nullptr;
   bool copied = false;
-  Activation(const void* p, int dtype, int rows_, int cols_, bool scaled, Scratch& s)
-      : src(p), f32(dtype == K3_DTYPE_F32), rows(rows_), cols(cols_) {
+  Activation(const void* p, int dtype, int rows_, int cols_, bool scaled, bool along, Scratch& s)
+      : src(p), f32(dtype == K3_DTYPE_F32), rows(rows_), cols(cols_), rows_out(rows_) {
     pitch = round_up((uint32_t)cols * 2, 16);
-    if (f32) {
-      planes = s.take(3ull * rows * pitch);
-      if (scaled) xs = reinterpret_cast<float*>(s.take(4ull * rows));
-    } else {
-      copied = pitch != (uint32_t)cols * 2 || !aligned16(p);
-      if (copied) planes = s.take((uint64_t)rows * pitch);
-    }
+    copied = f32 || pitch != (uint32_t)cols * 2 || !aligned16(p);
+    if (!copied) return;
+    if (along) rows_out = (int)round_up((uint32_t)rows, kStep);
+    planes = s.take((uint64_t)terms() * rows_out * pitch);
+    if (f32 && scaled) xs = reinterpret_cast<float*>(s.take(4ull * rows));
   }
   int terms() const { return f32 ? 3 : 1; }
   const uint8_t* plane(int t) const {
-    if (!f32 && !copied) return static_cast<const uint8_t*>(src);
-    return planes + (uint64_t)t * rows * pitch;
+    if (!copied) return static_cast<const uint8_t*>(src);
+    return planes + (uint64_t)t * rows_out * pitch;
   }
   int fill(hipStream_t st) const {
-    if (f32) return split_rows(src, planes, xs, rows, cols, pitch, st);
-    return copied ? pack_rows(src, planes, 2, rows, cols, pitch, st) : K3_SPINE_OK;
+    if (f32) return split_rows(src, planes, xs, rows, cols, rows_out, pitch, st);
+    return copied ? pack_rows(src, planes, 2, rows, cols, rows_out, pitch, st) : K3_SPINE_OK;
   }
 };
 
 // Tiles and the split of K.
 struct Plan {
-  bool large;
+  int bm;  // positions of a tile (its other side is kTileN)
   int tiles_n, tiles_m, splits, per, pitch;
   float* part;
 };
 
-constexpr int kLargeN = 256, kLargeM = 256, kSmallN = 128, kSmallM = 128;
+constexpr int kTileN = 256;
 
+// The tile and the split of K with the smallest estimated time.  One workgroup fills a CU,
+// so tiles run in rounds of as many as there are CUs; a round costs its steps, more for a
+// taller tile though less per output, and about six microseconds around them; a split K
+// costs writing and reading its partial sums and a launch.  Microseconds a step, measured
+// on products that fill the card: 1.6 at 256 positions, 0.93 at 128; 128 x 128 tiles,
+// two on a CU, took 1.1 for twice that output and lost to 256 x 128 at every size tried
+// (7168 x 6144 int8 at 1024 positions 106 against 92 us; 256 x 256 in two splits 97).
 Plan plan_product(int n, int m, int steps, bool glu, Scratch& s) {
-  const int cus = 256;
-  const int cols = glu ? (int)round_up((uint32_t)n, 16) * 2 : n;
-  Plan p{};
-  auto tiles = [&](int bn, int bm) {
-    return (int64_t)((cols + bn - 1) / bn) * ((m + bm - 1) / bm);
+  struct Shape {
+    int bm;
+    double us;
   };
-  p.large = tiles(kLargeN, kLargeM) >= 192;
-  const int bn = p.large ? kLargeN : kSmallN, bm = p.large ? kLargeM : kSmallM;
-  p.tiles_n = (cols + bn - 1) / bn;
-  p.tiles_m = (m + bm - 1) / bm;
-  const int64_t slots = p.large ? cus : 2 * cus;
-  const int64_t t = tiles(bn, bm);
-  int64_t splits = std::max<int64_t>(1, std::min<int64_t>(slots / std::max<int64_t>(t, 1), steps / 8));
+  static const Shape kShapes[] = {{256, 1.6}, {128, 0.93}};
+  const int cols = glu ? (int)round_up((uint32_t)n, 16) * 2 : n;
+  const int cus = std::max(1, device_cu_count());
   steps = std::max(steps, 1);
-  p.per = (int)((steps + splits - 1) / splits);
-  p.splits = (steps + p.per - 1) / p.per;
+  Plan p{};
+  double best = 0;
+  for (const Shape& t : kShapes) {
+    const int64_t tiles = (int64_t)((cols + kTileN - 1) / kTileN) * ((m + t.bm - 1) / t.bm);
+    for (int want = 1; want <= 32 && (want == 1 || want * 4 <= steps); ++want) {
+      const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
+      const double rounds = (double)((tiles * splits + cus - 1) / cus);
+      double us = rounds * (per * t.us + 6.0);
+      if (splits > 1) us += 4.0 + 8.0 * splits * (double)m * cols / 5e6;
+      if (best != 0 && us >= best) continue;
+      best = us;
+      p.bm = t.bm;
+      p.per = per;
+      p.splits = splits;
+    }
+  }
+  p.tiles_n = (cols + kTileN - 1) / kTileN;
+  p.tiles_m = (m + p.bm - 1) / p.bm;
   p.pitch = (int)round_up((uint32_t)cols, 4);
-  if (p.splits > 1)
-    p.part = reinterpret_cast<float*>(s.take(4ull * p.splits * m * p.pitch));
-  else
-    p.part = nullptr;
+  if (p.splits > 1) p.part = reinterpret_cast<float*>(s.take(4ull * p.splits * m * p.pitch));
   return p;
 }
 
@@ -469,12 +608,12 @@ int product(GemmArgs a, const Epilogue& e, const Plan& p, const char* what, hipS
     TimedLaunch tl(KC_SPINE_MFMA, st);
     const dim3 grid((unsigned)tiles, (unsigned)p.splits);
     float* part = p.splits > 1 ? p.part : nullptr;
-    if (p.large)
-      launch_timed(tl, (k_gemm<kLargeN, kLargeM, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e,
-                   part, p.pitch);
+    if (p.bm == 256)
+      launch_timed(tl, (k_gemm<kTileN, 256, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e, part,
+                   p.pitch);
     else
-      launch_timed(tl, (k_gemm<kSmallN, kSmallM, 2, 2, WL, XL, EPI>), grid, dim3(256), 0, st, a, e,
-                   part, p.pitch);
+      launch_timed(tl, (k_gemm<kTileN, 128, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e, part,
+                   p.pitch);
     const int rc = launched_or(tl, what);
     if (rc != K3_SPINE_OK) return rc;
   }
@@ -547,8 +686,8 @@ struct LinearCall {
   LinearCall(const K3HipLinearV1& op, void* ws)
       : s(ws),
         w(op.weights, op.matrix_kind == K3_SPINE_MATRIX_INT8 ? 1 : 2, (int)op.rows,
-          (int)op.columns, s),
-        x(op.x, (int)op.x_dtype, (int)op.positions, (int)op.columns, true, s),
+          (int)op.columns, false, s),
+        x(op.x, (int)op.x_dtype, (int)op.positions, (int)op.columns, true, false, s),
         p(plan_product((int)op.rows, (int)op.positions, x.terms() * steps_of((int)op.columns),
                        false, s)) {}
 };
@@ -561,34 +700,38 @@ struct GatedCall {
   GatedCall(const K3HipGatedV1& op, void* ws)
       : s(ws),
         g(op.gate, op.matrix_kind == K3_SPINE_MATRIX_INT8 ? 1 : 2, (int)op.rows, (int)op.columns,
-          s),
-        u(op.up, g.elem, g.rows, g.cols, s),
-        x(op.x, (int)op.x_dtype, (int)op.positions, (int)op.columns, true, s),
+          false, s),
+        u(op.up, g.elem, g.rows, g.cols, false, s),
+        x(op.x, (int)op.x_dtype, (int)op.positions, (int)op.columns, true, false, s),
         p(plan_product((int)op.rows, (int)op.positions, x.terms() * steps_of((int)op.columns),
                        true, s)) {}
 };
 
 // The products of the gradient: d_x over the 2 terms() segments of (dg, gate) and
-// (du, up), and both weight gradients as one product of 2 half rows.
+// (du, up), and both weight gradients as one product of 2 half rows.  dg and du are written
+// here, so their rows and columns can be whole steps of either product's K; whether a K
+// is follows from the other operand (k_x, k_w).
 struct GradCall {
   Scratch s;
   Matrix g, u;
   Activation x;
-  int half, terms;
+  int half, terms, rows_out, k_x, k_w;
   uint16_t* planes;
   Plan px, pw;
   GradCall(const K3HipGatedGradV1& op, void* ws)
       : s(ws),
-        g(op.gate, 2, (int)op.rows, (int)op.columns, s),
-        u(op.up, 2, (int)op.rows, (int)op.columns, s),
-        x(op.x, (int)op.dtype, (int)op.positions, (int)op.columns, false, s),
-        half((int)round_up(op.rows, 8)),
+        g(op.gate, 2, (int)op.rows, (int)op.columns, true, s),
+        u(op.up, 2, (int)op.rows, (int)op.columns, true, s),
+        x(op.x, (int)op.dtype, (int)op.positions, (int)op.columns, false, true, s),
+        half((int)round_up(op.rows, g.rows_out == u.rows_out && g.rows_out % kStep == 0 ? kStep : 8)),
         terms(x.terms()),
-        planes(reinterpret_cast<uint16_t*>(s.take(4ull * terms * op.positions * half))),
-        px(plan_product((int)op.columns, (int)op.positions,
-                        2 * terms * steps_of((int)op.rows), false, s)),
-        pw(plan_product((int)op.columns, 2 * half,
-                        (terms == 3 ? 6 : 1) * steps_of((int)op.positions), false, s)) {}
+        rows_out(x.rows_out),
+        k_x(std::min(g.rows_out, u.rows_out)),
+        k_w(x.rows_out),
+        planes(reinterpret_cast<uint16_t*>(s.take(4ull * terms * rows_out * half))),
+        px(plan_product((int)op.columns, (int)op.positions, 2 * terms * steps_of(k_x), false, s)),
+        pw(plan_product((int)op.columns, 2 * half, (terms == 3 ? 6 : 1) * steps_of(k_w), false,
+                        s)) {}
 };
 
 }  // namespace
@@ -693,21 +836,25 @@ int dense_gated_grad(const K3HipGatedGradV1& op, void* ws, hipStream_t st) {
   if (rc != K3_SPINE_OK) return rc;
   {
     TimedLaunch tl(KC_ACTIVATE, st);
-    const dim3 grid(grid_for((uint64_t)P * c.half));
+    const dim3 grid(grid_for((uint64_t)c.rows_out * (c.half / 8)));
+    const int vec = ((uint64_t)S * (f32 ? 4 : 2)) % 16 == 0 && aligned16(op.g) &&
+                    aligned16(op.u) && aligned16(op.grad);
     if (f32)
       launch_timed(tl, (k_gated_grad<float, 3>), grid, dim3(256), 0, st,
                    static_cast<const float*>(op.g), static_cast<const float*>(op.u),
-                   static_cast<const float*>(op.grad), c.planes, P, S, c.half, (int)op.activation);
+                   static_cast<const float*>(op.grad), c.planes, P, S, c.rows_out, c.half,
+                   (int)op.activation, vec);
     else
       launch_timed(tl, (k_gated_grad<uint16_t, 1>), grid, dim3(256), 0, st,
                    static_cast<const uint16_t*>(op.g), static_cast<const uint16_t*>(op.u),
-                   static_cast<const uint16_t*>(op.grad), c.planes, P, S, c.half,
-                   (int)op.activation);
+                   static_cast<const uint16_t*>(op.grad), c.planes, P, S, c.rows_out, c.half,
+                   (int)op.activation, vec);
     if ((rc = launched_or(tl, what)) != K3_SPINE_OK) return rc;
   }
   const uint32_t ldd = 4u * (uint32_t)c.half;  // bytes of a row of dg and du
   auto plane = [&](int t, int which) {
-    return reinterpret_cast<const uint8_t*>(c.planes) + (uint64_t)t * P * ldd + 2ull * which * c.half;
+    return reinterpret_cast<const uint8_t*>(c.planes) + (uint64_t)t * c.rows_out * ldd +
+           2ull * which * c.half;
   };
   GemmArgs a{};
   for (int t = c.terms - 1; t >= 0; --t)
@@ -718,8 +865,7 @@ int dense_gated_grad(const K3HipGatedGradV1& op, void* ws, hipStream_t st) {
     }
   a.n = H;
   a.m = P;
-  a.k = S;
-  a.kw = S;
+  a.k = a.kw = c.k_x;
   a.kx = c.half;
   a.ldw = c.g.pitch;
   a.ldx = ldd;
@@ -743,7 +889,7 @@ int dense_gated_grad(const K3HipGatedGradV1& op, void* ws, hipStream_t st) {
   }
   b.n = H;
   b.m = 2 * c.half;
-  b.k = b.kw = b.kx = P;
+  b.k = b.kw = b.kx = c.k_w;
   b.ldw = c.x.pitch;
   b.ldx = ldd;
   Epilogue f{};
