@@ -168,7 +168,9 @@ struct Tile {
         k = kChunkK * (L == L_INT8 ? slot ^ int8_swizzle(rl) : slot ^ kmajor_swizzle(rl));
       }
       const uint8_t* b = kPairs && (j / (L == L_INT8 ? 1 : 2)) % 2 ? base2 : base;
-      load_lds(k < left ? b + off[i] : reinterpret_cast<const uint8_t*>(&g_zero_chunk),
+      uint32_t o = off[i];
+      asm volatile("" : "+v"(o));  // its 64-bit form lives here, not across the main loop
+      load_lds(k < left ? b + o : reinterpret_cast<const uint8_t*>(&g_zero_chunk),
                lds + 1024 * j);
     }
   }
