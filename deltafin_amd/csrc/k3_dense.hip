@@ -549,33 +549,35 @@ struct Activation {
 
 // Tiles and the split of K.
 struct Plan {
-  int bm;  // positions of a tile (its other side is kTileN)
+  int bn, bm;  // rows of the matrix and positions of a tile
   int tiles_n, tiles_m, splits, per, pitch;
   float* part;
 };
 
-constexpr int kTileN = 256;
-
 // The tile and the split of K with the smallest estimated time.  One workgroup fills a CU,
 // so tiles run in rounds of as many as there are CUs; a round costs its steps, more for a
-// taller tile though less per output, and about six microseconds around them; a split K
+// larger tile though less per output, and about six microseconds around them; a split K
 // costs writing and reading its partial sums and a launch.  Microseconds a step, measured
-// on products that fill the card: 1.6 at 256 positions, 0.93 at 128; 128 x 128 tiles,
-// two on a CU, took 1.1 for twice that output and lost to 256 x 128 at every size tried
-// (7168 x 6144 int8 at 1024 positions 106 against 92 us; 256 x 256 in two splits 97).
+// on products that fill the card.  224 rows serve products that leave the last round of
+// 256 half empty (4096 x 7168 outputs: 448 tiles of 256, 512 of 224, on 256 CUs; the
+// gated block's pairs of 16 rows need an even number of blocks per wave and do without).
+// 128 x 128 tiles, two on a CU, took 1.1 us for twice that output and lost to 256 x 128 at
+// every size tried (7168 x 6144 int8 at 1024 positions 106 against 92 us; 256 x 256 in two
+// splits 97).
 Plan plan_product(int n, int m, int steps, bool glu, Scratch& s) {
   struct Shape {
-    int bm;
+    int bn, bm;
     double us;
   };
-  static const Shape kShapes[] = {{256, 1.6}, {128, 0.93}};
+  static const Shape kShapes[] = {{256, 256, 1.6}, {256, 128, 0.93}, {224, 256, 1.44}};
   const int cols = glu ? (int)round_up((uint32_t)n, 16) * 2 : n;
   const int cus = std::max(1, device_cu_count());
   steps = std::max(steps, 1);
   Plan p{};
   double best = 0;
   for (const Shape& t : kShapes) {
-    const int64_t tiles = (int64_t)((cols + kTileN - 1) / kTileN) * ((m + t.bm - 1) / t.bm);
+    if (glu && t.bn == 224) continue;
+    const int64_t tiles = (int64_t)((cols + t.bn - 1) / t.bn) * ((m + t.bm - 1) / t.bm);
     for (int want = 1; want <= 32 && (want == 1 || want * 4 <= steps); ++want) {
       const int per = (steps + want - 1) / want, splits = (steps + per - 1) / per;
       const double rounds = (double)((tiles * splits + cus - 1) / cus);
@@ -583,12 +585,13 @@ Plan plan_product(int n, int m, int steps, bool glu, Scratch& s) {
       if (splits > 1) us += 4.0 + 8.0 * splits * (double)m * cols / 5e6;
       if (best != 0 && us >= best) continue;
       best = us;
+      p.bn = t.bn;
       p.bm = t.bm;
       p.per = per;
       p.splits = splits;
     }
   }
-  p.tiles_n = (cols + kTileN - 1) / kTileN;
+  p.tiles_n = (cols + p.bn - 1) / p.bn;
   p.tiles_m = (m + p.bm - 1) / p.bm;
   p.pitch = (int)round_up((uint32_t)cols, 4);
   if (p.splits > 1) p.part = reinterpret_cast<float*>(s.take(4ull * p.splits * m * p.pitch));
@@ -608,12 +611,17 @@ int product(GemmArgs a, const Epilogue& e, const Plan& p, const char* what, hipS
     TimedLaunch tl(KC_SPINE_MFMA, st);
     const dim3 grid((unsigned)tiles, (unsigned)p.splits);
     float* part = p.splits > 1 ? p.part : nullptr;
-    if (p.bm == 256)
-      launch_timed(tl, (k_gemm<kTileN, 256, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e, part,
+    if (p.bn == 224) {
+      if constexpr (EPI != EPI_GLU)
+        launch_timed(tl, (k_gemm<224, 256, 2, 4, WL, XL, EPI>), grid, dim3(512), 0, st, a, e, part,
+                     p.pitch);
+    } else if (p.bm == 256) {
+      launch_timed(tl, (k_gemm<256, 256, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e, part,
                    p.pitch);
-    else
-      launch_timed(tl, (k_gemm<kTileN, 128, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e, part,
+    } else {
+      launch_timed(tl, (k_gemm<256, 128, 4, 2, WL, XL, EPI>), grid, dim3(512), 0, st, a, e, part,
                    p.pitch);
+    }
     const int rc = launched_or(tl, what);
     if (rc != K3_SPINE_OK) return rc;
   }

@@ -197,9 +197,8 @@ struct Frags {
   bf16x8 v[2][F];
   u32x4 raw[L == L_INT8 ? F : 1];  // both halves' int8 values as read
 
-  // Where this lane reads block row16 of a tile in half kk.  Opaque, so that it is formed
-  // here each time instead of being held (or, NMAJOR, F of its exclusive-ors being held)
-  // in registers across the loop, which spilled.
+  // Where this lane reads in half kk, formed anew for each: block row16 of the tile, or
+  // (NMAJOR) block 0, whose chunk number another block's number is exclusive-or'ed into.
   template <int kk>
   __device__ static __forceinline__ uint32_t place(int row16, int lane) {
     const int i16 = lane & 15, g = lane >> 4;
@@ -210,21 +209,22 @@ struct Frags {
       at = row16 * 1024 + i16 * 64 + ((g ^ int8_swizzle(i16)) << 4);
     } else {
       const int kr = 16 * g + 8 * kk + (i16 >> 2);  // and kr + 4: the same swizzle
-      at = kr * (2 * R) + (i16 & 3) * 8 + ((row16 ^ nmajor_swizzle<R>(kr)) << 5);
+      at = kr * (2 * R) + (i16 & 3) * 8 + (nmajor_swizzle<R>(kr) << 5);  // of block 0
     }
     return at;
   }
 
-  // Block f of half kk, `at` being place<kk>.  int8 blocks come whole with the first half.
+  // Block f from row16 on of half kk, `at` being place<kk>.  int8 blocks come whole with the
+  // first half.
   template <int kk>
-  __device__ __forceinline__ void read(int f, const uint8_t* tile, uint32_t at) {
+  __device__ __forceinline__ void read(int f, const uint8_t* tile, uint32_t at, int row16) {
     if constexpr (L == L_KMAJOR) {
       v[kk][f] = *reinterpret_cast<const bf16x8*>(tile + at + 2048 * f);
     } else if constexpr (L == L_INT8) {
       if constexpr (kk == 0) raw[f] = *reinterpret_cast<const u32x4*>(tile + at + 1024 * f);
     } else {
       typedef __attribute__((address_space(3))) s16x4 lds_s16x4;
-      const uint8_t* q = tile + (at ^ (f << 5));
+      const uint8_t* q = tile + (at ^ ((uint32_t)(row16 + f) << 5));
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)q);
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(q + 8 * R));
       const bf16x4 a = __builtin_bit_cast(bf16x4, lo), b = __builtin_bit_cast(bf16x4, hi);
@@ -263,7 +263,9 @@ template <int BN, int BM, int NWN, int NWM, int WL, int XL, bool kPairs>
 struct Core {
   static constexpr int kWaves = NWN * NWM;
   static constexpr int FN = BN / 16 / NWN, FM = BM / 16 / NWM;
-  typedef Tile<BN, WL, kWaves, kPairs> TW;
+  // rows that the weight side's tile has in LDS: a power of two
+  static constexpr int kRowsW = BN <= 128 ? 128 : 256;
+  typedef Tile<kRowsW, WL, kWaves, kPairs> TW;
   typedef Tile<BM, XL, kWaves, false> TX;
   static_assert(TW::kLoads % kWaves == 0 && TX::kLoads % kWaves == 0, "equal shares of loads");
   // Three tiles of the weight side and two of the other: 160 KB, all of a CU's LDS, at 256 x
@@ -317,7 +319,7 @@ struct Core {
       px += dx;
       if (--leftx == 0 && ++segx < a.segments) open_x(0);
     };
-    typedef Frags<BN, WL, FN> FW;
+    typedef Frags<kRowsW, WL, FN> FW;
     typedef Frags<BM, XL, FM> FX;
     FW fw;
     FX fx;
@@ -326,9 +328,9 @@ struct Core {
                     uint32_t at_x) {
       constexpr int kk = decltype(half)::value;
       if (b < FN)
-        fw.template read<kk>(b, tw_at, at_w);
+        fw.template read<kk>(b, tw_at, at_w, wn * FN);
       else
-        fx.template read<kk>(b - FN, tx_at, at_x);
+        fx.template read<kk>(b - FN, tx_at, at_x, wm * FM);
     };
     // Half kk's products, a column of FN at a time; between the columns go the loads of
     // later steps, then the reads of the other half, few at a time: 64 loads of 1 KB issued

@@ -79,7 +79,8 @@ def _ints(rng, shape, lo, hi):
 
 @pytest.mark.parametrize("positions,rows,cols", [(1, 7168, 2048), (9, 896, 7168), (48, 3584, 7168),
                                                  (100, 7168, 6144), (517, 2050, 7168),
-                                                 (1024, 7168, 2048), (2100, 6144, 1003)])
+                                                 (1024, 7168, 2048), (2048, 7168, 208),
+                                                 (2100, 6144, 1003)])
 @pytest.mark.parametrize("kind", ["bf16", "int8"])
 @pytest.mark.parametrize("x_dt", ["f32", "bf16"])
 def test_linear_integers_are_exact(gpu, positions, rows, cols, kind, x_dt):
@@ -266,7 +267,8 @@ def test_gated_backward(gpu, positions, rows, cols, dt, act):
 
 
 @pytest.mark.parametrize("positions,rows,cols", [(4096, 264, 2050), (1000, 2048, 1536),
-                                                 (517, 1003, 2050)])
+                                                 (517, 1003, 2050), (2048, 136, 7168),
+                                                 (200, 1024, 7168)])
 @pytest.mark.parametrize("dt", ["f32", "bf16"])
 def test_gated_backward_integers_are_exact(gpu, positions, rows, cols, dt):
     """g = 0 makes SiLU's dg = grad u / 2 and du = 0, g = 100 makes dg = grad u and du =
