@@ -12,6 +12,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "k3_dense.h"
 #include "k3_device.h"
@@ -43,9 +44,16 @@ struct Epilogue {
   int vec;            // four neighbours of a row are one aligned access
 };
 
+// The nearest BF16 values, as a pair with a's low (finite values that round past the largest
+// become infinite).
 __device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
   typedef float v2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_convertvector(v2{a, b}, v2bf));
+}
+
+// Value i of a pair.
+__device__ __forceinline__ float head_of(uint32_t pair, int i) {
+  return __uint_as_float(i ? pair & 0xffff0000u : pair << 16);
 }
 
 // Columns n .. n + 3 (those below e.n) of a row that starts at element `row`.
@@ -87,10 +95,39 @@ __device__ __forceinline__ f32x4 load4(const Epilogue& e, const void* p, int bf1
   return v;
 }
 
-// Sums v (GLU: of gate, u of up) of row m, columns n .. n + 3.
+// What columns n .. n + 3 have in common over the rows.
+struct Columns {
+  f32x4 rs, rs2, bias;
+};
 template <int EPI>
-__device__ __forceinline__ void finish(const Epilogue& e, int m, int n, f32x4 v, f32x4 u) {
-  if (n >= e.n || m >= e.m) return;
+__device__ __forceinline__ Columns load_columns(const Epilogue& e, int n) {
+  Columns c{};
+  if constexpr (EPI != EPI_GRAD) {
+    if (e.rs) c.rs = load4(e, e.rs, 0, 0, n);
+    if (EPI == EPI_GLU && e.rs) c.rs2 = load4(e, e.rs2, 0, 0, n);
+    if (EPI == EPI_LINEAR && e.bias) c.bias = load4(e, e.bias, 0, 0, n);
+  }
+  return c;
+}
+// What a row adds to them, requested ahead of its use.
+struct RowInputs {
+  f32x4 res;
+  float xs;
+};
+template <int EPI>
+__device__ __forceinline__ RowInputs load_row(const Epilogue& e, int m, int n) {
+  RowInputs r{};
+  if constexpr (EPI != EPI_GRAD) {
+    if (e.xs) r.xs = e.xs[m];
+    if (EPI == EPI_LINEAR && e.res) r.res = load4(e, e.res, e.bf16, (uint64_t)m * e.n, n);
+  }
+  return r;
+}
+
+// Sums v (GLU: of gate, u of up) of row m < e.m, columns n .. n + 3 of which n < e.n.
+template <int EPI>
+__device__ __forceinline__ void finish(const Epilogue& e, const Columns& c, const RowInputs& in,
+                                       int m, int n, f32x4 v, f32x4 u) {
   if constexpr (EPI == EPI_GRAD) {
     void* out = e.out;
     int r = m;
@@ -106,13 +143,12 @@ __device__ __forceinline__ void finish(const Epilogue& e, int m, int n, f32x4 v,
   }
   const uint64_t row = (uint64_t)m * e.n;
   if (e.xs) {
-    const float s = e.xs[m];
-    v *= s;
-    if constexpr (EPI == EPI_GLU) u *= s;
+    v *= in.xs;
+    if constexpr (EPI == EPI_GLU) u *= in.xs;
   }
   if (e.rs) {
-    v *= load4(e, e.rs, 0, 0, n);
-    if constexpr (EPI == EPI_GLU) u *= load4(e, e.rs2, 0, 0, n);
+    v *= c.rs;
+    if constexpr (EPI == EPI_GLU) u *= c.rs2;
   }
   if constexpr (EPI == EPI_GLU) {
     f32x4 h;
@@ -124,13 +160,111 @@ __device__ __forceinline__ void finish(const Epilogue& e, int m, int n, f32x4 v,
     }
     store4(e, e.out, row, n, h);
   } else {
-    if (e.bias) v += load4(e, e.bias, 0, 0, n);
+    if (e.bias) v += c.bias;
     if (e.act != K3_DENSE_ACT_NONE) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) v[i] = unary_activation(e.act, v[i]);
     }
-    if (e.res) v += load4(e, e.res, e.bf16, row, n);
+    if (e.res) v += in.res;
     store4(e, e.out, row, n, v);
+  }
+}
+
+// A whole wave's part of a tile where all of it exists and four neighbours are one access:
+// a column or two of sums (16 rows each) at a time, with the next ones' residual on its way
+// (sum after sum, it took 40 of 304 us at 4096 x 7168 x 6144; all of it ahead spilled).
+// n0, m0: this lane's first column and row; a sum's are n0 + 16 i and m0 + 16 j.
+template <int EPI, bool kBf16, bool kInt8, int FN, int FM>
+__device__ __forceinline__ void finish_inside(const Epilogue& e, int n0, int m0,
+                                              const f32x4 (&acc)[FN][FM]) {
+  constexpr bool kGlu = EPI == EPI_GLU;
+  constexpr int kOut = kGlu ? FN / 2 : FN;  // blocks of 16 outputs
+  typedef typename std::conditional<kBf16, uint2, f32x4>::type Quad;  // four outputs
+  auto store = [&](void* out, uint64_t at, f32x4 v) {
+    if constexpr (kBf16)
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
+          make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
+    else
+      *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = v;
+  };
+  f32x4 rs[FN], bias[FN];
+  if constexpr (EPI != EPI_GRAD) {
+    const f32x4 ones = {1.f, 1.f, 1.f, 1.f}, none = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+      const int n = n0 + 16 * (kGlu ? i / 2 : i);
+      rs[i] = kInt8 ? *reinterpret_cast<const f32x4*>((kGlu && i % 2 ? e.rs2 : e.rs) + n) : ones;
+      bias[i] = !kGlu && e.bias ? *reinterpret_cast<const f32x4*>(e.bias + n) : none;
+    }
+  }
+  constexpr bool kRes = EPI == EPI_LINEAR;
+  constexpr int kCols = FN > 4 ? 1 : 2;  // columns at a time
+  Quad res[2][kCols][kRes ? FN : 1];
+  float xs[2][kCols];
+  auto request = [&](int c) {  // of columns kCols c and behind
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) {
+      const int m = m0 + 16 * (kCols * c + k);
+      if constexpr (EPI != EPI_GRAD) xs[c & 1][k] = e.xs ? e.xs[m] : 1.f;
+      if constexpr (kRes) {
+        if (e.res) {
+#pragma unroll
+          for (int i = 0; i < FN; ++i)
+            res[c & 1][k][i] = *reinterpret_cast<const Quad*>(
+                static_cast<const uint8_t*>(e.res) +
+                ((uint64_t)m * e.n + n0 + 16 * i) * (kBf16 ? 2 : 4));
+        }
+      }
+    }
+  };
+  request(0);
+#pragma unroll
+  for (int c = 0; c < FM / kCols; ++c) {
+    if (c + 1 < FM / kCols) request(c + 1);
+#pragma unroll
+    for (int k = 0; k < kCols; ++k) {
+      const int j = kCols * c + k;
+      const uint64_t at = (uint64_t)(m0 + 16 * j) * e.n + n0;
+#pragma unroll
+      for (int i = 0; i < kOut; ++i) {
+        if constexpr (EPI == EPI_GRAD) {
+          if (e.half)
+            finish<EPI>(e, Columns{}, RowInputs{}, m0 + 16 * j, n0 + 16 * i, acc[i][j], f32x4{});
+          else
+            store(e.out, at + 16 * i, acc[i][j]);
+        } else if constexpr (kGlu) {
+          f32x4 g = acc[2 * i][j] * xs[c & 1][k], u = acc[2 * i + 1][j] * xs[c & 1][k];
+          if constexpr (kInt8) {
+            g *= rs[2 * i];
+            u *= rs[2 * i + 1];
+          }
+          f32x4 h;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) h[q] = activate(e.act, g[q], u[q]);
+          if (e.out1) {
+            store(e.out1, at + 16 * i, g);
+            store(e.out2, at + 16 * i, u);
+          }
+          store(e.out, at + 16 * i, h);
+        } else {
+          f32x4 v = acc[i][j] * xs[c & 1][k];
+          if constexpr (kInt8) v *= rs[i];
+          if (e.bias) v += bias[i];
+          if (e.act != K3_DENSE_ACT_NONE) {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = unary_activation(e.act, v[q]);
+          }
+          if (e.res) {
+            const Quad r = res[c & 1][k][i];
+            if constexpr (kBf16)
+              v += f32x4{head_of(r.x, 0), head_of(r.x, 1), head_of(r.y, 0), head_of(r.y, 1)};
+            else
+              v += r;
+          }
+          store(e.out, at + 16 * i, v);
+        }
+      }
+    }
   }
 }
 
@@ -147,34 +281,46 @@ __global__ __launch_bounds__(64 * NWN * NWM) void k_gemm(const GemmArgs a, const
   f32x4 acc[C::FN][C::FM];
   C::run(a, lds, tn, tm, blockIdx.y, acc);
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int nb = tn * BN + (wave % NWN) * C::FN * 16 + 4 * (lane >> 4);  // GLU: of pair columns
-  const int mb = tm * BM + (wave / NWN) * C::FM * 16 + (lane & 15);
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nw = tn * BN + (wave % NWN) * C::FN * 16;  // the wave's first (GLU: pair) column
+  const int mw = tm * BM + (wave / NWN) * C::FM * 16;
+  const int n0 = (kGlu && !part ? nw / 2 : nw) + 4 * (lane >> 4), m0 = mw + (lane & 15);
   if (part) {
 #pragma unroll
     for (int j = 0; j < C::FM; ++j) {
-      const int m = mb + 16 * j;
+      const int m = m0 + 16 * j;
       if (m >= a.m) continue;
       float* row = part + ((uint64_t)blockIdx.y * a.m + m) * pitch;
 #pragma unroll
       for (int i = 0; i < C::FN; ++i)
-        if (nb + 16 * i < pitch) *reinterpret_cast<f32x4*>(row + nb + 16 * i) = acc[i][j];
+        if (n0 + 16 * i < pitch) *reinterpret_cast<f32x4*>(row + n0 + 16 * i) = acc[i][j];
     }
     return;
   }
-  if constexpr (kGlu) {
-    const int n0 = (tn * BN + (wave % NWN) * C::FN * 16) / 2 + 4 * (lane >> 4);
+  constexpr int kBlocks = kGlu ? C::FN / 2 : C::FN;
+  if (e.vec && mw + 16 * C::FM <= e.m && (kGlu ? nw / 2 : nw) + 16 * kBlocks <= e.n) {
+    if (e.bf16)
+      finish_inside<EPI, true, WL == L_INT8>(e, n0, m0, acc);
+    else
+      finish_inside<EPI, false, WL == L_INT8>(e, n0, m0, acc);
+    return;
+  }
 #pragma unroll
-    for (int j = 0; j < C::FM; ++j)
+  for (int j = 0; j < C::FM; ++j) {
+    const int m = m0 + 16 * j;
+    if (m >= e.m) continue;
 #pragma unroll
-      for (int i = 0; i < C::FN; i += 2)
-        finish<EPI>(e, mb + 16 * j, n0 + 8 * i, acc[i][j], acc[i + 1][j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < C::FM; ++j)
-#pragma unroll
-      for (int i = 0; i < C::FN; ++i)
-        finish<EPI>(e, mb + 16 * j, nb + 16 * i, acc[i][j], f32x4{});
+    for (int i = 0; i < kBlocks; ++i) {
+      const int n = n0 + 16 * i;
+      if (n >= e.n) continue;
+      const Columns c = load_columns<EPI>(e, n);
+      const RowInputs in = load_row<EPI>(e, m, n);
+      if constexpr (kGlu)
+        finish<EPI>(e, c, in, m, n, acc[2 * i][j], acc[2 * i + 1][j]);
+      else
+        finish<EPI>(e, c, in, m, n, acc[i][j], f32x4{});
+    }
   }
 }
 
@@ -188,13 +334,15 @@ __global__ __launch_bounds__(256) void k_gemm_join(const Epilogue e, const float
     const int m = (int)(t / quads), n = 4 * (int)(t % quads);
     const uint64_t at =
         (uint64_t)m * pitch + (EPI == EPI_GLU ? (uint32_t)(n >> 4) * 32 + (n & 15) : n);
+    const Columns c = load_columns<EPI>(e, n);
+    const RowInputs in = load_row<EPI>(e, m, n);
     f32x4 v = {0.f, 0.f, 0.f, 0.f}, u = {0.f, 0.f, 0.f, 0.f};
     for (int s = 0; s < splits; ++s) {
       const float* p = part + (uint64_t)s * e.m * pitch + at;
       v += *reinterpret_cast<const f32x4*>(p);
       if constexpr (EPI == EPI_GLU) u += *reinterpret_cast<const f32x4*>(p + 16);
     }
-    finish<EPI>(e, m, n, v, u);
+    finish<EPI>(e, c, in, m, n, v, u);
   }
 }
 
@@ -217,12 +365,6 @@ __device__ __forceinline__ void terms3(float v, uint32_t (&t)[3]) {
   const float r = v - __uint_as_float(t[0] << 16);
   t[1] = nearest_bf16(r);
   t[2] = nearest_bf16(r - __uint_as_float(t[1] << 16));
-}
-
-// The two nearest BF16 values, by the hardware's convert: finite ones that round past the
-// largest become infinite, so only for values scaled into [-2, 2].
-__device__ __forceinline__ float head_of(uint32_t pair, int i) {
-  return __uint_as_float(i ? pair & 0xffff0000u : pair << 16);
 }
 
 // fp32 rows to three planes [3][rows_out][pitch / 2] (pitch in bytes, zeros past cols and in
