@@ -175,17 +175,17 @@ __device__ __forceinline__ void finish(const Epilogue& e, const Columns& c, cons
 // (sum after sum, it took 40 of 304 us at 4096 x 7168 x 6144; all of it ahead spilled).
 // n0, m0: this lane's first column and row; a sum's are n0 + 16 i and m0 + 16 j.
 template <int EPI, bool kBf16, bool kInt8, int FN, int FM>
-__device__ __forceinline__ void finish_inside(const Epilogue& e, int n0, int m0,
+__device__ __forceinline__ void finish_inside(const Epilogue& e, void* out, int n0, int m0,
                                               const f32x4 (&acc)[FN][FM]) {
   constexpr bool kGlu = EPI == EPI_GLU;
   constexpr int kOut = kGlu ? FN / 2 : FN;  // blocks of 16 outputs
   typedef typename std::conditional<kBf16, uint2, f32x4>::type Quad;  // four outputs
-  auto store = [&](void* out, uint64_t at, f32x4 v) {
+  auto store = [&](void* to, uint64_t at, f32x4 v) {
     if constexpr (kBf16)
-      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(out) + at) =
+      *reinterpret_cast<uint2*>(static_cast<uint16_t*>(to) + at) =
           make_uint2(bf16_pair(v[0], v[1]), bf16_pair(v[2], v[3]));
     else
-      *reinterpret_cast<f32x4*>(static_cast<float*>(out) + at) = v;
+      *reinterpret_cast<f32x4*>(static_cast<float*>(to) + at) = v;
   };
   f32x4 rs[FN], bias[FN];
   if constexpr (EPI != EPI_GRAD) {
@@ -228,10 +228,7 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int n0, int m0,
 #pragma unroll
       for (int i = 0; i < kOut; ++i) {
         if constexpr (EPI == EPI_GRAD) {
-          if (e.half)
-            finish<EPI>(e, Columns{}, RowInputs{}, m0 + 16 * j, n0 + 16 * i, acc[i][j], f32x4{});
-          else
-            store(e.out, at + 16 * i, acc[i][j]);
+          store(out, at + 16 * i, acc[i][j]);
         } else if constexpr (kGlu) {
           f32x4 g = acc[2 * i][j] * xs[c & 1][k], u = acc[2 * i + 1][j] * xs[c & 1][k];
           if constexpr (kInt8) {
@@ -245,7 +242,7 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int n0, int m0,
             store(e.out1, at + 16 * i, g);
             store(e.out2, at + 16 * i, u);
           }
-          store(e.out, at + 16 * i, h);
+          store(out, at + 16 * i, h);
         } else {
           f32x4 v = acc[i][j] * xs[c & 1][k];
           if constexpr (kInt8) v *= rs[i];
@@ -261,7 +258,7 @@ __device__ __forceinline__ void finish_inside(const Epilogue& e, int n0, int m0,
             else
               v += r;
           }
-          store(e.out, at + 16 * i, v);
+          store(out, at + 16 * i, v);
         }
       }
     }
@@ -299,11 +296,17 @@ __global__ __launch_bounds__(64 * NWN * NWM) void k_gemm(const GemmArgs a, const
     return;
   }
   constexpr int kBlocks = kGlu ? C::FN / 2 : C::FN;
-  if (e.vec && mw + 16 * C::FM <= e.m && (kGlu ? nw / 2 : nw) + 16 * kBlocks <= e.n) {
+  // the wave's rows in its matrix (the second of a gradient's two starts at row `half`)
+  const bool second = EPI == EPI_GRAD && e.half && mw >= e.half;
+  const int first = second ? mw - e.half : mw;
+  const int rows = EPI == EPI_GRAD && e.half ? e.valid : e.m;
+  if (e.vec && first + 16 * C::FM <= rows && (kGlu ? nw / 2 : nw) + 16 * kBlocks <= e.n) {
+    void* out = second ? e.out1 : e.out;
+    const int r0 = first + (lane & 15);
     if (e.bf16)
-      finish_inside<EPI, true, WL == L_INT8>(e, n0, m0, acc);
+      finish_inside<EPI, true, WL == L_INT8>(e, out, n0, r0, acc);
     else
-      finish_inside<EPI, false, WL == L_INT8>(e, n0, m0, acc);
+      finish_inside<EPI, false, WL == L_INT8>(e, out, n0, r0, acc);
     return;
   }
 #pragma unroll
