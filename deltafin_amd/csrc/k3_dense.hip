@@ -360,14 +360,17 @@ __device__ __forceinline__ uint32_t nearest_bf16(float v) {
   return (r & 0x7f80u) == 0x7f80u ? u >> 16 : r;
 }
 
-// Three BF16 terms of v; only the first of an infinity or NaN.
-__device__ __forceinline__ void terms3(float v, uint32_t (&t)[3]) {
-  t[0] = nearest_bf16(v);
-  t[1] = t[2] = 0u;
-  if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) return;
-  const float r = v - __uint_as_float(t[0] << 16);
-  t[1] = nearest_bf16(r);
-  t[2] = nearest_bf16(r - __uint_as_float(t[1] << 16));
+// Three BF16 terms of a and of b as pairs; only the first of an infinity or NaN.  The
+// hardware's convert rounds values of the last half step under infinity to it: those take
+// the slow way.
+__device__ __forceinline__ void terms3(float a, float b, uint32_t (&t)[3]) {
+  t[0] = bf16_pair(a, b);
+  const float most = fmaxf(fabsf(a), fabsf(b));
+  if (!(most < 0x1.fep+127f)) t[0] = nearest_bf16(a) | nearest_bf16(b) << 16;
+  const float ra = fabsf(a) < INFINITY ? a - head_of(t[0], 0) : 0.f;
+  const float rb = fabsf(b) < INFINITY ? b - head_of(t[0], 1) : 0.f;
+  t[1] = bf16_pair(ra, rb);
+  t[2] = bf16_pair(ra - head_of(t[1], 0), rb - head_of(t[1], 1));
 }
 
 // fp32 rows to three planes [3][rows_out][pitch / 2] (pitch in bytes, zeros past cols and in
@@ -441,23 +444,10 @@ __global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x,
       u32x4 t[3];
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const float a = v[2 * q] * scale, b = v[2 * q + 1] * scale;
-        if constexpr (kScaled) {
-          const uint32_t t0 = bf16_pair(a, b);
-          // an infinity or NaN is its first term alone
-          const float ra = fabsf(a) < INFINITY ? a - head_of(t0, 0) : 0.f;
-          const float rb = fabsf(b) < INFINITY ? b - head_of(t0, 1) : 0.f;
-          const uint32_t t1 = bf16_pair(ra, rb);
-          t[0][q] = t0;
-          t[1][q] = t1;
-          t[2][q] = bf16_pair(ra - head_of(t1, 0), rb - head_of(t1, 1));
-        } else {
-          uint32_t lo[3], hi[3];
-          terms3(a, lo);
-          terms3(b, hi);
+        uint32_t p[3];
+        terms3(v[2 * q] * scale, v[2 * q + 1] * scale, p);
 #pragma unroll
-          for (int i = 0; i < 3; ++i) t[i][q] = lo[i] | hi[i] << 16;
-        }
+        for (int i = 0; i < 3; ++i) t[i][q] = p[i];
       }
 #pragma unroll
       for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4*>(d + i * plane + 16ull * g) = t[i];
@@ -542,33 +532,36 @@ __global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, con
     load8(u + at, vec, n, uv);
     load8(grad + at, vec, n, dv);
     u32x4 og[TERMS], ou[TERMS];
+    float dg[8], du[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      float dg = 0.f, du = 0.f;
+      dg[i] = du[i] = 0.f;
       if (i < n) {
         const float sig = 1.0f / (1.0f + expf(-gv[i]));
         if (act == K3_ACT_SILU) {
-          dg = dv[i] * uv[i] * (sig * (1.0f + gv[i] * (1.0f - sig)));
-          du = dv[i] * (gv[i] * sig);
+          dg[i] = dv[i] * uv[i] * (sig * (1.0f + gv[i] * (1.0f - sig)));
+          du[i] = dv[i] * (gv[i] * sig);
         } else {
           const float a = tanhf(gv[i] / 4.0f), b = tanhf(uv[i] / 25.0f);
-          dg = dv[i] * (25.0f * b) * ((1.0f - a * a) * sig + 4.0f * a * (sig * (1.0f - sig)));
-          du = dv[i] * (4.0f * a * sig) * (1.0f - b * b);
+          dg[i] = dv[i] * (25.0f * b) * ((1.0f - a * a) * sig + 4.0f * a * (sig * (1.0f - sig)));
+          du[i] = dv[i] * (4.0f * a * sig) * (1.0f - b * b);
         }
       }
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
       uint32_t tg[3], tu[3];
       if constexpr (TERMS == 1) {
-        const uint32_t both = bf16_pair(dg, du);
-        tg[0] = both & 0xffffu;
-        tu[0] = both >> 16;
+        tg[0] = bf16_pair(dg[2 * q], dg[2 * q + 1]);
+        tu[0] = bf16_pair(du[2 * q], du[2 * q + 1]);
       } else {
-        terms3(dg, tg);
-        terms3(du, tu);
+        terms3(dg[2 * q], dg[2 * q + 1], tg);
+        terms3(du[2 * q], du[2 * q + 1], tu);
       }
 #pragma unroll
       for (int k = 0; k < TERMS; ++k) {
-        og[k][i / 2] = i % 2 ? og[k][i / 2] | tg[k] << 16 : tg[k];
-        ou[k][i / 2] = i % 2 ? ou[k][i / 2] | tu[k] << 16 : tu[k];
+        og[k][q] = tg[k];
+        ou[k][q] = tu[k];
       }
     }
     uint16_t* o = planes + row * 2 * half + c;
@@ -696,6 +689,7 @@ struct Activation {
 struct Plan {
   int bn, bm;  // rows of the matrix and positions of a tile
   int tiles_n, tiles_m, splits, per, pitch;
+  double us;  // its estimated time
   float* part;
 };
 
@@ -729,7 +723,7 @@ Plan plan_product(int n, int m, int steps, bool glu, Scratch& s) {
       double us = rounds * (per * t.us + 6.0);
       if (splits > 1) us += 4.0 + 8.0 * splits * (double)m * cols / 5e6;
       if (best != 0 && us >= best) continue;
-      best = us;
+      p.us = best = us;
       p.bn = t.bn;
       p.bm = t.bm;
       p.per = per;
@@ -788,10 +782,23 @@ bool vec_ok(int n, int out_elem, std::initializer_list<const void*> ptrs) {
 }
 
 // Few positions: the skinny kernels stream a matrix once per 16 positions with no scratch
-// memory and no second launch.
-constexpr int kSkinnyPositions = 16;
+// memory and no second launch.  Up to 16 positions they always win; beyond, where their
+// time, about 0.22 us (fp32 rows: 0.3) per million weights and 16 positions behind a
+// launch, is under the tiles': us on skinny / tiled kernels 7168 x 2048 bf16 at 32 positions
+// 9.9 / 14.4 and at 128 27 / 19, fp32 rows 12 / 23 and 40 / 33; 7168 x 6144 fp32 rows at 32
+// positions 27 / 41 and at 64 51 / 43; 1024 x 1024 at 128 positions 9.8 / 12.8.
+constexpr int kSkinnyAlways = 16, kSkinnyMost = 512;
+bool skinny_pays(int n, int m, int k, int x_dtype, bool glu) {
+  if (m <= kSkinnyAlways) return true;
+  if (m > kSkinnyMost) return false;
+  const bool f32 = x_dtype == K3_DTYPE_F32;
+  const double weights = (double)n * k * (glu ? 2 : 1) * 1e-6;
+  const double skinny = 8.0 + (f32 ? 0.30 : 0.22) * weights * ((m + 15) / 16);
+  Scratch none(nullptr);
+  return skinny <= plan_product(n, m, (f32 ? 3 : 1) * steps_of(k), glu, none).us + (f32 ? 4.0 : 0.0);
+}
 bool skinny_linear(const K3HipLinearV1& op, SkinnyOp* sk) {
-  if (op.positions > kSkinnyPositions) return false;
+  if (op.positions > kSkinnyMost) return false;
   sk->kind = op.matrix_kind == K3_SPINE_MATRIX_INT8 ? SKINNY_INT8 : SKINNY_BF16;
   sk->w = op.weights;
   sk->row_scales = op.row_scales;
@@ -805,10 +812,10 @@ bool skinny_linear(const K3HipLinearV1& op, SkinnyOp* sk) {
   sk->rows = (int)op.rows;
   sk->cols = (int)op.columns;
   sk->positions = (int)op.positions;
-  return skinny_fits(*sk);
+  return skinny_fits(*sk) && skinny_pays(sk->rows, sk->positions, sk->cols, sk->x_dtype, false);
 }
 bool skinny_gated(const K3HipGatedV1& op, SkinnyOp* sk) {
-  if (op.positions > kSkinnyPositions) return false;
+  if (op.positions > kSkinnyMost) return false;
   sk->kind = op.matrix_kind == K3_SPINE_MATRIX_INT8 ? SKINNY_INT8 : SKINNY_BF16;
   sk->w = op.gate;
   sk->w2 = op.up;
@@ -824,7 +831,7 @@ bool skinny_gated(const K3HipGatedV1& op, SkinnyOp* sk) {
   sk->rows = (int)op.rows;
   sk->cols = (int)op.columns;
   sk->positions = (int)op.positions;
-  return skinny_fits(*sk);
+  return skinny_fits(*sk) && skinny_pays(sk->rows, sk->positions, sk->cols, sk->x_dtype, true);
 }
 int run_skinny(const SkinnyOp& sk, const char* what, hipStream_t st) {
   if (launch_skinny(sk, KC_SPINE_MFMA, st) == K3_HIP_OK) return K3_SPINE_OK;

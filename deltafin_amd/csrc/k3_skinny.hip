@@ -79,6 +79,7 @@ struct SkinnyArgs {
   int S, per;     // waves splitting the lines, lines of a wave
   int out_bf16, act;
   int unary;  // K3_DENSE_ACT_* of a single product
+  int mix;    // GLU by mixed tiles
 };
 
 // BF16 activation rows in blocks of 64 columns, as many as a BF16 weight line has (the
@@ -289,11 +290,14 @@ __device__ __forceinline__ void plain_dots(const uint8_t* w, const uint8_t* sc, 
 }
 
 // RQ quads of activation rows per workgroup: 4 RQ positions (1..16 of a
-// 16-column block, or 32).
-template <int kW, typename XT, int RQ, int TL, bool kGlu, int D>
+// 16-column block, or 32).  kMix (GLU): a tile's two loads of 8 rows are 8 gate and the same
+// 8 up rows, so that few rows give twice the workgroups.
+template <int kW, typename XT, int RQ, int TL, bool kGlu, int D, bool kMix>
 __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args) {
+  static_assert(!kMix || (kGlu && TL == 1 && kW != SKINNY_FP4), "one mixed tile");
   constexpr int Q = operands<kW>();
-  constexpr int TLT = kGlu ? 2 * TL : TL;
+  constexpr int TLT = kGlu && !kMix ? 2 * TL : TL;
+  constexpr int RT = kMix ? 8 : 16 * TL;  // outputs of a position
   constexpr int NB = RQ > 4 ? RQ / 4 : 1;       // 16-position column blocks
   constexpr int NT = sizeof(XT) == 4 ? 3 : 1;   // terms of an activation
   constexpr int OB = block_operands<XT>();
@@ -308,7 +312,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int i16 = lane & 15, g = lane >> 4;
   const bool odd = (i16 & 1) != 0;
-  const int r0 = blockIdx.x * 16 * TL;
+  const int r0 = blockIdx.x * RT;
   const int p0 = blockIdx.y * 4 * RQ;
   const int rows = args.rows, P = args.P, S = args.S;
   const uint32_t row_bytes = kW == SKINNY_BF16   ? 2u * args.cols
@@ -328,7 +332,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
   for (int t = 0; t < TL; ++t) {
 #pragma unroll
     for (int h = 0; h < 2; ++h)
-      aoff[t][h] = (uint32_t)min(16 * t + 8 * h + (i16 >> 1), last) * row_bytes + piece;
+      aoff[t][h] =
+          (uint32_t)min((kMix ? 0 : 16 * t + 8 * h) + (i16 >> 1), last) * row_bytes + piece;
     if constexpr (kW == SKINNY_FP4)
       soff[t] = (uint32_t)min(16 * t + 8 * (i16 & 1) + (i16 >> 1), last) * (uint32_t)G;
   }
@@ -375,7 +380,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
     for (int t = 0; t < TLT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        s.a[t][h] = load_chunk(wb[t / TL] + 128u * (uint32_t)j + (aoff[t % TL][h] - back));
+        s.a[t][h] = load_chunk(wb[kMix ? h : t / TL] + 128u * (uint32_t)j +
+                               (aoff[t % TL][h] - back));
   };
   // Block b of a stage into the wave's LDS region.  16-byte piece c of row r is
   // at slot 16 r + (c ^ r % 16) (raw) or, of each term, 8 r + (c ^ (r / 2) % 8), so
@@ -520,19 +526,20 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
   __syncthreads();
   const int np = min(4 * RQ, P - p0);
   const float* pf = reinterpret_cast<const float*>(sums);
-  const int n_out = 16 * TL * np;
+  const int n_out = RT * np;
   for (int o0 = 64 * wave; o0 < n_out; o0 += 64 * S) {
     const int o = min(o0 + lane, n_out - 1);
-    const int rt = o % (16 * TL), p = o / (16 * TL);
+    const int rt = o % RT, p = o / RT;
     const int row = r0 + rt;
     const bool stored = o0 + lane < n_out && row < rows;
-    const int t = rt >> 4, wr = rt & 15;
-    const int m = wr < 8 ? 2 * wr : 2 * wr - 15;  // MFMA row of weight row wr
-    const int at = (t * NB + (p >> 4)) * 256 + (16 * (m >> 2) + (p & 15)) * 4 + (m & 3);
     float v[kGlu ? 2 : 1];
 #pragma unroll
     for (int k = 0; k < (kGlu ? 2 : 1); ++k) {
-      const float* pk = pf + at + k * TL * NB * 256;
+      const int t = (kMix ? 0 : rt >> 4) + (kMix ? 0 : k * TL);
+      const int wr = kMix ? rt + 8 * k : rt & 15;
+      const int m = wr < 8 ? 2 * wr : 2 * wr - 15;  // MFMA row of weight row wr
+      const float* pk =
+          pf + (t * NB + (p >> 4)) * 256 + (16 * (m >> 2) + (p & 15)) * 4 + (m & 3);
       float sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kMaxWaves; ++w)  // wave order; all reads in flight at once
@@ -541,14 +548,14 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
       uint64_t left = __ballot(stored && !(fabsf(sum) < INFINITY));
       while (left != 0) {
         const int first = __builtin_ctzll(left);
-        const int bp = (o0 + first) / (16 * TL);
+        const int bp = (o0 + first) / RT;
         int bit[4], brow[4];
         float again[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int b = left != 0 ? __builtin_ctzll(left) : first;
-          bit[i] = (o0 + b) / (16 * TL) == bp ? b : first;
-          brow[i] = r0 + (o0 + bit[i]) % (16 * TL);
+          bit[i] = (o0 + b) / RT == bp ? b : first;
+          brow[i] = r0 + (o0 + bit[i]) % RT;
           left &= ~(1ull << bit[i]);
         }
         plain_dots<kW, XT>(args.w[k], args.sc[k],
@@ -589,17 +596,18 @@ __global__ __launch_bounds__(64 * kMaxWaves) void k_skinny(const SkinnyArgs args
   }
 }
 
-template <int kW, typename XT, int RQ, int TL, bool kGlu, int D>
+template <int kW, typename XT, int RQ, int TL, bool kGlu, int D, bool kMix = false>
 bool go(const SkinnyArgs& a, hipStream_t st, TimedLaunch& tl) {
-  constexpr int TLT = kGlu ? 2 * TL : TL;
+  constexpr int TLT = kGlu && !kMix ? 2 * TL : TL;
+  constexpr int RT = kMix ? 8 : 16 * TL;
   constexpr int NB = RQ > 4 ? RQ / 4 : 1;
   constexpr int kRegions = line_blocks<kW, XT>() > 1 ? 2 : 1;
   const unsigned lds = (unsigned)(a.S * (TLT * NB * 64 + kRegions * block_f4<XT, RQ>()) *
                                   sizeof(f32x4));
-  const void* fn = reinterpret_cast<const void*>(k_skinny<kW, XT, RQ, TL, kGlu, D>);
+  const void* fn = reinterpret_cast<const void*>(k_skinny<kW, XT, RQ, TL, kGlu, D, kMix>);
   if (!lds_fits(fn, 64 * a.S, lds)) return false;
-  const dim3 grid((a.rows + 16 * TL - 1) / (16 * TL), (a.P + 4 * RQ - 1) / (4 * RQ));
-  launch_timed(tl, (k_skinny<kW, XT, RQ, TL, kGlu, D>), grid, dim3(64 * a.S), lds, st, a);
+  const dim3 grid((a.rows + RT - 1) / RT, (a.P + 4 * RQ - 1) / (4 * RQ));
+  launch_timed(tl, (k_skinny<kW, XT, RQ, TL, kGlu, D, kMix>), grid, dim3(64 * a.S), lds, st, a);
   return true;
 }
 
@@ -640,6 +648,9 @@ bool go_rows(int TL, const SkinnyArgs& a, hipStream_t st, TimedLaunch& tl) {
 // workgroups than CUs (MXFP4, with its longer lines, always one).
 template <int kW, typename XT, int RQ>
 bool go_glu_tiles(int TL, const SkinnyArgs& a, hipStream_t st, TimedLaunch& tl) {
+  if constexpr (std::is_same<XT, Bf16Row64>::value) {
+    if (a.mix) return go<kW, XT, RQ, 1, true, 2, true>(a, st, tl);
+  }
   if constexpr (kW != SKINNY_FP4)
     if (TL > 1) return go<kW, XT, RQ, 2, true, 2>(a, st, tl);
   return go<kW, XT, RQ, 1, true, depth<kW, 2>()>(a, st, tl);
@@ -719,6 +730,7 @@ int launch_skinny(const SkinnyOp& op, int kernel_class, hipStream_t st) {
   const int pb = (a.P + 15) / 16;
   int TL = 1;
   while (TL < 4 && (int64_t)((a.rows + 16 * TL - 1) / (16 * TL)) * pb > cus) TL *= 2;
+  a.mix = 2 * ((a.rows + 15) / 16) * pb <= cus;
   TimedLaunch tl(kernel_class, st);
   bool ok;
   const bool glu = op.w2 != nullptr;

@@ -34,7 +34,7 @@ def _check(t: torch.Tensor, dtypes, shape, what: str) -> None:
     if fits and t.shape == shape and t.is_contiguous():
         at = t.get_device()
         if at >= 0:
-            if at == torch.cuda.current_device():
+            if at == torch._C._cuda_getDevice():
                 return
             raise ValueError(f"{what} is on {t.device}, the current device is "
                              f"cuda:{torch.cuda.current_device()}")

@@ -97,11 +97,11 @@ def test_grad_refusals(kw, match):
 def test_workspace_refusals(name, make):
     from deltafin_amd import _lib
     lib = _lib.load()
-    need = getattr(lib, name + "_workspace_bytes")(C.byref(make(positions=50)))
+    need = getattr(lib, name + "_workspace_bytes")(C.byref(make(positions=50, columns=100)))
     assert need > _lib.K3_DENSE_NO_WORKSPACE
-    _refused(name, make(positions=50), "workspace", ws=None)
-    _refused(name, make(positions=50), "workspace", ws=256 * A + 16)
-    _refused(name, make(positions=50), "workspace", bytes_=need - 1)
+    _refused(name, make(positions=50, columns=100), "workspace", ws=None)
+    _refused(name, make(positions=50, columns=100), "workspace", ws=256 * A + 16)
+    _refused(name, make(positions=50, columns=100), "workspace", bytes_=need - 1)
     _refused(name, None, "null descriptor")
     assert getattr(lib, name + "_workspace_bytes")(None) == 0
     assert getattr(lib, name + "_workspace_bytes")(C.byref(make(rows=0))) == 0

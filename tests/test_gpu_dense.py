@@ -48,7 +48,8 @@ def _close(found, want, bound, dtype, tag):
 
 
 SHAPES = [(1, 7, 5), (1, 64, 128), (3, 130, 72), (17, 1, 64), (64, 257, 600), (65, 16, 1),
-          (129, 136, 344), (200, 513, 33), (300, 96, 520)]
+          (129, 136, 344), (200, 513, 33), (300, 96, 520),
+          (520, 96, 520), (530, 257, 72)]
 
 
 @pytest.mark.parametrize("positions,rows,cols", SHAPES)
@@ -199,7 +200,8 @@ def test_linear_non_finite_rows_stay_their_own(gpu, x_dt, positions):
     _close(out[2:], clean[2:], bound[2:], x_dt, "other rows")
 
 
-GATED = [(1, 16, 8), (1, 40, 264), (5, 33, 70), (70, 130, 128), (131, 200, 328), (300, 64, 65)]
+GATED = [(1, 16, 8), (1, 40, 264), (5, 33, 70), (70, 130, 128), (131, 200, 328), (300, 64, 65),
+         (515, 48, 264)]
 
 
 @pytest.mark.parametrize("positions,rows,cols", GATED)
