@@ -39,10 +39,11 @@ constexpr double kVanish = 64.0;     // weights under 2^-kVanish round to none
 constexpr int kRanges = 4;           // top-k's, top-p's, min-p's and the draw's
 constexpr int kSmall = 64;           // tokens that one wave orders
 
-// The ranges of bins in which a row's positions lie, apart and ascending.
+// The ranges of bins in which a row's positions lie; a bin's tokens are gathered for the
+// first of them that holds it.
 struct RowPlan {
   int32_t first;                     // lowest index of the largest logit (T not above 0)
-  int32_t ranges;
+  int32_t listed;                    // places of the list in use
   int32_t b0[kRanges], b1[kRanges];  // first and last bin
   int32_t base[kRanges];             // place of the first in the list, or -1
   int32_t pad[2];
@@ -132,46 +133,46 @@ __device__ __forceinline__ void fill_table(double* table) {
 }
 
 // Calls f(logit, index) for the tokens [t0, t1) of a row, each thread of the workgroup its
-// share: 16 bytes per load where they lie inside, single tokens at ragged ends.
+// share: 16 bytes per load, four in flight (those past the end repeat the last, so that none
+// is conditional: behind a branch each waited for the one before), single tokens ahead of
+// the first 16-byte boundary and behind the last.
 template <typename T, typename F>
 __device__ __forceinline__ void scan(const T* row, int t0, int t1, int threads, F f) {
   constexpr int kPer = 16 / (int)sizeof(T);
   constexpr int kUnroll = 4;
   const T* p = row + t0;
-  const int n = t1 - t0;
-  const int lead = (int)(((uintptr_t)p & 15u) / sizeof(T));  // tokens of the first chunk before p
-  const int chunks = (lead + n + kPer - 1) / kPer;
-  const u32x4* base = reinterpret_cast<const u32x4*>(p - lead);
-  auto value = [](u32x4 v, int i) {
-    if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
-    return __uint_as_float(i % 2 ? v[i / 2] & 0xffff0000u : v[i / 2] << 16);
+  const int n = max(t1 - t0, 0);
+  const int off = (int)(((uintptr_t)p & 15u) / sizeof(T));
+  const int head = min(n, off ? kPer - off : 0);
+  const int chunks = (n - head) / kPer;
+  auto one = [&](int t) {
+    float l;
+    if constexpr (sizeof(T) == 4)
+      l = p[t];
+    else
+      l = bf16_bits_to_f32(p[t]);
+    f(l, t0 + t);
   };
+  const int tail = head + chunks * kPer;
+  if ((int)threadIdx.x < head) one(threadIdx.x);
+  if ((int)threadIdx.x < n - tail) one(tail + threadIdx.x);
+  const u32x4* base = reinterpret_cast<const u32x4*>(p + head);
   for (int c0 = threadIdx.x; c0 < chunks; c0 += kUnroll * threads) {
     u32x4 v[kUnroll];
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int c = c0 + k * threads;
-      const bool whole = c * kPer >= lead && (c + 1) * kPer <= lead + n;
-      if (whole) v[k] = base[c];
-    }
+    for (int k = 0; k < kUnroll; ++k) v[k] = base[min(c0 + k * threads, chunks - 1)];
 #pragma unroll
     for (int k = 0; k < kUnroll; ++k) {
       const int c = c0 + k * threads;
-      const bool whole = c * kPer >= lead && (c + 1) * kPer <= lead + n;
-      if (whole) {
+      if (c >= chunks) break;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) f(value(v[k], i), t0 + c * kPer + i - lead);
-      } else if (c < chunks) {
-        for (int i = 0; i < kPer; ++i) {
-          const int t = c * kPer + i - lead;
-          if (t < 0 || t >= n) continue;
-          float l;
-          if constexpr (sizeof(T) == 4)
-            l = p[t];
-          else
-            l = bf16_bits_to_f32(p[t]);
-          f(l, t0 + t);
-        }
+      for (int i = 0; i < kPer; ++i) {
+        float l;
+        if constexpr (sizeof(T) == 4)
+          l = __uint_as_float(v[k][i]);
+        else
+          l = __uint_as_float(i % 2 ? v[k][i / 2] & 0xffff0000u : v[k][i / 2] << 16);
+        f(l, t0 + head + c * kPer + i);
       }
     }
   }
@@ -462,54 +463,48 @@ __global__ __launch_bounds__(kScanThreads) void k_sample_gather(const SampleArgs
   }
   b0[3] = h.crossing(false, lo ? draw_target(l, lo) : 0);
   b1[3] = h.crossing(false, draw_target(l, hi));
+  // places, while they fit, for ranges that no earlier one holds
+  int base[kRanges], total = 0;
+#pragma unroll
+  for (int i = 0; i < kRanges; ++i) {
+    base[i] = -1;
+    bool held = b1[i] < 0;
+#pragma unroll
+    for (int k = 0; k < i; ++k) held = held || (base[k] >= 0 && b0[k] <= b0[i] && b1[i] <= b1[k]);
+    if (held) continue;
+    const int n = (int)(h.count[b1[i]] - h.count_before(b0[i]));
+    if (n > kList - total) continue;
+    base[i] = total;
+    total += n;
+  }
+  const int wave = threadIdx.x >> 6;
+  static_assert(2 * kRanges <= kScanThreads / 64, "a wave per end of a range");
+#pragma unroll
+  for (int i = 0; i < kRanges; ++i) {
+    if (wave != i && wave != kRanges + i) continue;
+    // (an empty range of values where there is none)
+    float* end = wave == i ? &most[i] : &least[i];
+    const float none = wave == i ? -INFINITY : INFINITY;
+    const float v = base[i] < 0 ? none
+                    : wave == i ? value_of(last_key(r, b0[i] - 1) + 1)
+                                : value_of(last_key(r, b1[i]));
+    if ((threadIdx.x & 63) == 0) *end = v;
+  }
   if (threadIdx.x == 0) {
-    // ascending, joined where they meet, and given places while they fit
-    int n = 0, total = 0;
-    int at = -1;
-    for (;;) {
-      int f = kBins, e = -1;  // the next range: the smallest first bin behind `at`
-#pragma unroll
-      for (int i = 0; i < kRanges; ++i)
-        if (b1[i] > at && max(b0[i], at + 1) < f) f = max(b0[i], at + 1);
-      if (f == kBins) break;
-      e = f - 1;
-      for (int again = 0; again < kRanges; ++again)
-#pragma unroll
-        for (int i = 0; i < kRanges; ++i)
-          if (b0[i] <= e + 1 && b1[i] > e && b1[i] >= f) e = b1[i];
-      const int tokens_in = (int)(h.count[e] - h.count_before(f));
-      plan.b0[n] = f;
-      plan.b1[n] = e;
-      plan.base[n] = total + tokens_in <= kList ? total : -1;
-      if (plan.base[n] >= 0) total += tokens_in;
-      ++n;
-      at = e;
-      if (n == kRanges) break;
-    }
-    plan.ranges = n;
-    for (int i = n; i < kRanges; ++i) {
-      plan.b0[i] = kBins;
-      plan.b1[i] = plan.base[i] = -1;
-    }
     plan.first = a.vocab;
+    plan.listed = total;
+#pragma unroll
+    for (int i = 0; i < kRanges; ++i) {
+      plan.b0[i] = b0[i];
+      plan.b1[i] = b1[i];
+      plan.base[i] = base[i];
+    }
     found = 0;
   }
   __syncthreads();
-  static_assert(kRanges <= kScanThreads / 64, "a wave per range");
-  const int wave = threadIdx.x >> 6;
-  if (wave < kRanges) {
-    const bool any = plan.base[wave] >= 0;
-    const uint32_t from = any ? last_key(r, plan.b0[wave] - 1) + 1 : 0u;
-    const uint32_t to = any ? last_key(r, plan.b1[wave]) : 0u;
-    if ((threadIdx.x & 63) == 0) {
-      most[wave] = any && from <= to ? value_of(from) : -INFINITY;
-      least[wave] = any && from <= to ? value_of(to) : INFINITY;
-    }
-  }
   if (part == 0 && threadIdx.x < sizeof(RowPlan) / 4)
     reinterpret_cast<int32_t*>(&a.plan[row])[threadIdx.x] =
         reinterpret_cast<const int32_t*>(&plan)[threadIdx.x];
-  __syncthreads();
   float m[kRanges], s[kRanges];
 #pragma unroll
   for (int i = 0; i < kRanges; ++i) {
@@ -531,10 +526,14 @@ __global__ __launch_bounds__(kScanThreads) void k_sample_gather(const SampleArgs
   // found, their round trips took most of the launch
   for (uint32_t i = threadIdx.x; i < min(found, (uint32_t)kList); i += kScanThreads) {
     const int b = bin_of(r, log2_weight(r, value_of(key[i])));
-    int in = 0;
-    for (int k = 0; k < plan.ranges; ++k)
-      if (plan.b0[k] <= b && b <= plan.b1[k]) in = k;
-    const uint32_t at = plan.base[in] + (h.count_before(b) - h.count_before(plan.b0[in])) +
+    int from = 0, place = 0;
+#pragma unroll
+    for (int k = kRanges - 1; k >= 0; --k)
+      if (base[k] >= 0 && b0[k] <= b && b <= b1[k]) {
+        from = b0[k];
+        place = base[k];
+      }
+    const uint32_t at = place + (h.count_before(b) - h.count_before(from)) +
                         atomicAdd(&a.taken[(uint64_t)row * kBins + b], 1u);
     if (at < (uint32_t)kList) a.list[(uint64_t)row * kList + at] = make_uint2(key[i], index[i]);
   }
@@ -583,7 +582,8 @@ struct Picker {
   };
   __device__ __forceinline__ Place place(int bin) const {
     Place p{0, -1, 0.f, 0.f};
-    for (int i = 0; i < sh.plan.ranges; ++i)
+#pragma unroll
+    for (int i = kRanges - 1; i >= 0; --i)
       if (sh.plan.b0[i] <= bin && bin <= sh.plan.b1[i] && sh.plan.base[i] >= 0) {
         const uint32_t before = sh.h.count_before(bin);
         p.at = sh.plan.base[i] + (int)(before - sh.h.count_before(sh.plan.b0[i]));
@@ -799,12 +799,7 @@ __global__ __launch_bounds__(kPickThreads) void k_sample_pick(const SampleArgs a
     reinterpret_cast<int32_t*>(&sh.plan)[threadIdx.x] =
         reinterpret_cast<const int32_t*>(&a.plan[ri])[threadIdx.x];
   sh.h.load(a, ri);
-  int listed = 0;
-  for (int i = 0; i < sh.plan.ranges; ++i)
-    if (sh.plan.base[i] >= 0)
-      listed = sh.plan.base[i] +
-               (int)(sh.h.count[sh.plan.b1[i]] - sh.h.count_before(sh.plan.b0[i]));
-  for (int i = threadIdx.x; i < min(listed, kList); i += kPickThreads)
+  for (int i = threadIdx.x; i < min(sh.plan.listed, kList); i += kPickThreads)
     sh.list[i] = a.list[(uint64_t)ri * kList + i];
   Picker<T> p{sh, a, row, r};
   const Limits l = row_limits(a, ri, sh.h);
