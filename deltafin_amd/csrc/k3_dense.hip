@@ -86,11 +86,15 @@ __device__ __forceinline__ f32x4 load4(const Epilogue& e, const void* p, int bf1
     return f32x4{__uint_as_float(b.x << 16), __uint_as_float(b.x & 0xffff0000u),
                  __uint_as_float(b.y << 16), __uint_as_float(b.y & 0xffff0000u)};
   }
+  // n < e.n; loads past the row's end repeat its last value (unconditional, as in
+  // k_pack_rows) and are not used
+  if (bf16) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if (n + i >= e.n) break;
-    v[i] = bf16 ? __uint_as_float((uint32_t) static_cast<const uint16_t*>(p)[row + n + i] << 16)
-                : static_cast<const float*>(p)[row + n + i];
+    for (int i = 0; i < 4; ++i)
+      v[i] = bf16_bits_to_f32(static_cast<const uint16_t*>(p)[row + min(n + i, e.n - 1)]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = static_cast<const float*>(p)[row + min(n + i, e.n - 1)];
   }
   return v;
 }
@@ -388,7 +392,7 @@ __global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x,
   __shared__ float red[4];
   const int groups = (int)(pitch / 16);
   for (int row = blockIdx.x; row < rows_out; row += gridDim.x) {
-    const float* p = x + (uint64_t)row * cols;
+    const float* p = x + (uint64_t)min(row, rows - 1) * cols;
     auto load = [&](int g, float (&v)[8]) {
       const int c = 8 * g;
       if (row < rows && aligned && c + 8 <= cols) {
@@ -400,7 +404,10 @@ __global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x,
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = row < rows && c + i < cols ? p[c + i] : 0.f;
+        for (int i = 0; i < 8; ++i) {
+          const float value = p[min(c + i, cols - 1)];  // unconditional, as in k_pack_rows
+          v[i] = row < rows && c + i < cols ? value : 0.f;
+        }
       }
     };
     float held[kHeld][8];
@@ -477,11 +484,14 @@ __global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u3
   for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
     const uint64_t row = t / chunks;
     const int c0 = row < (uint64_t)rows ? (int)(t - row * chunks) * kPer : cols;
-    const T* p = src + row * cols;
+    const T* p = src + min(row, (uint64_t)rows - 1) * cols;
     u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
-      const uint32_t b = c0 + i < cols ? (uint32_t)p[c0 + i] : 0u;
+      // (loads past the end repeat the last value: behind a condition each would wait for
+      // the one before)
+      const uint32_t value = p[min(c0 + i, cols - 1)];
+      const uint32_t b = c0 + i < cols ? value : 0u;
       v[i * (int)sizeof(T) / 4] |= b << (8 * ((i * (int)sizeof(T)) & 3));
     }
     dst[t] = v;
@@ -494,12 +504,13 @@ __global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u3
 __device__ __forceinline__ float widen(uint16_t b) { return bf16_bits_to_f32(b); }
 __device__ __forceinline__ float widen(float f) { return f; }
 
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, bool vec, int n, float (&v)[8]) {
-  if (vec && n >= 8) {
+// The first W values from p, n of which exist (n < 1: p is any value, none counts).
+template <typename T, int W>
+__device__ __forceinline__ void load_row_part(const T* p, bool vec, int n, float (&v)[W]) {
+  if (W == 8 && vec && n >= 8) {
     constexpr int kPer = 16 / (int)sizeof(T);
 #pragma unroll
-    for (int h = 0; h < 8 / kPer; ++h) {
+    for (int h = 0; h < W / kPer; ++h) {
       const u32x4 q = *reinterpret_cast<const u32x4*>(p + kPer * h);
 #pragma unroll
       for (int i = 0; i < kPer; ++i)
@@ -508,33 +519,37 @@ __device__ __forceinline__ void load8(const T* p, bool vec, int n, float (&v)[8]
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? widen(p[i]) : 0.f;
+    for (int i = 0; i < W; ++i) {
+      const float value = widen(p[max(min(i, n - 1), 0)]);  // unconditional, as in k_pack_rows
+      v[i] = i < n ? value : 0.f;
+    }
   }
 }
 
-// Eight neighbouring columns per thread.
-template <typename T, int TERMS>
+// W neighbouring columns per thread: eight, or two where eight would leave the card to a few
+// waves that each go through eight sets of exponentials (517 x 1003 fp32 12 us of 105).
+template <typename T, int TERMS, int W>
 __global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, const T* __restrict__ u,
                                                     const T* __restrict__ grad,
                                                     uint16_t* __restrict__ planes, int rows,
                                                     int cols, int rows_out, int half, int act,
                                                     int vec) {
   const uint64_t plane = (uint64_t)rows_out * 2 * half;
-  const uint32_t groups = (uint32_t)half / 8;
+  const uint32_t groups = (uint32_t)half / W;
   const uint64_t total = (uint64_t)rows_out * groups;
   for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
     const uint64_t row = t / groups;
-    const int c = 8 * (int)(t - row * groups);
+    const int c = W * (int)(t - row * groups);
     const int n = row < (uint64_t)rows ? cols - c : 0;
-    const uint64_t at = row * cols + c;
-    float gv[8], uv[8], dv[8];
-    load8(g + at, vec, n, gv);
-    load8(u + at, vec, n, uv);
-    load8(grad + at, vec, n, dv);
-    u32x4 og[TERMS], ou[TERMS];
-    float dg[8], du[8];
+    const uint64_t at = n > 0 ? row * cols + c : 0;
+    float gv[W], uv[W], dv[W];
+    load_row_part<T, W>(g + at, vec, n, gv);
+    load_row_part<T, W>(u + at, vec, n, uv);
+    load_row_part<T, W>(grad + at, vec, n, dv);
+    uint32_t og[TERMS][W / 2], ou[TERMS][W / 2];
+    float dg[W], du[W];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+    for (int i = 0; i < W; ++i) {
       dg[i] = du[i] = 0.f;
       if (i < n) {
         const float sig = 1.0f / (1.0f + expf(-gv[i]));
@@ -549,7 +564,7 @@ __global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, con
       }
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
+    for (int q = 0; q < W / 2; ++q) {
       uint32_t tg[3], tu[3];
       if constexpr (TERMS == 1) {
         tg[0] = bf16_pair(dg[2 * q], dg[2 * q + 1]);
@@ -567,8 +582,14 @@ __global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, con
     uint16_t* o = planes + row * 2 * half + c;
 #pragma unroll
     for (int k = 0; k < TERMS; ++k) {
-      *reinterpret_cast<u32x4*>(o + k * plane) = og[k];
-      *reinterpret_cast<u32x4*>(o + k * plane + half) = ou[k];
+      if constexpr (W == 8) {
+        *reinterpret_cast<u32x4*>(o + k * plane) = u32x4{og[k][0], og[k][1], og[k][2], og[k][3]};
+        *reinterpret_cast<u32x4*>(o + k * plane + half) =
+            u32x4{ou[k][0], ou[k][1], ou[k][2], ou[k][3]};
+      } else {
+        *reinterpret_cast<uint32_t*>(o + k * plane) = og[k][0];
+        *reinterpret_cast<uint32_t*>(o + k * plane + half) = ou[k][0];
+      }
     }
   }
 }
@@ -996,19 +1017,23 @@ int dense_gated_grad(const K3HipGatedGradV1& op, void* ws, hipStream_t st) {
   if (rc != K3_SPINE_OK) return rc;
   {
     TimedLaunch tl(KC_ACTIVATE, st);
-    const dim3 grid(grid_for((uint64_t)c.rows_out * (c.half / 8)));
     const int vec = ((uint64_t)S * (f32 ? 4 : 2)) % 16 == 0 && aligned16(op.g) &&
                     aligned16(op.u) && aligned16(op.grad);
+    const uint64_t eights = (uint64_t)c.rows_out * (c.half / 8);
+    const bool wide = eights >= 1024ull * std::max(1, device_cu_count());
+    const dim3 grid(grid_for(wide ? eights : 4 * eights));
+    auto go = [&](auto kernel, auto* type) {
+      typedef typename std::remove_pointer<decltype(type)>::type T;
+      launch_timed(tl, kernel, grid, dim3(256), 0, st, static_cast<const T*>(op.g),
+                   static_cast<const T*>(op.u), static_cast<const T*>(op.grad), c.planes, P, S,
+                   c.rows_out, c.half, (int)op.activation, vec);
+    };
+    float* f = nullptr;
+    uint16_t* h = nullptr;
     if (f32)
-      launch_timed(tl, (k_gated_grad<float, 3>), grid, dim3(256), 0, st,
-                   static_cast<const float*>(op.g), static_cast<const float*>(op.u),
-                   static_cast<const float*>(op.grad), c.planes, P, S, c.rows_out, c.half,
-                   (int)op.activation, vec);
+      wide ? go(k_gated_grad<float, 3, 8>, f) : go(k_gated_grad<float, 3, 2>, f);
     else
-      launch_timed(tl, (k_gated_grad<uint16_t, 1>), grid, dim3(256), 0, st,
-                   static_cast<const uint16_t*>(op.g), static_cast<const uint16_t*>(op.u),
-                   static_cast<const uint16_t*>(op.grad), c.planes, P, S, c.rows_out, c.half,
-                   (int)op.activation, vec);
+      wide ? go(k_gated_grad<uint16_t, 1, 8>, h) : go(k_gated_grad<uint16_t, 1, 2>, h);
     if ((rc = launched_or(tl, what)) != K3_SPINE_OK) return rc;
   }
   const uint32_t ldd = 4u * (uint32_t)c.half;  // bytes of a row of dg and du
