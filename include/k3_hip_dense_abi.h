@@ -33,9 +33,11 @@
  * the sum; products are exact and sums are fp32.  BF16 activations enter as they are;
  * fp32 ones as three BF16 terms, whose sum has all 24 bits.  Outputs are rounded once.
  * A result does not depend on what other calls ran, but may differ in its last bits
- * with the number of positions (the order of its sum goes by the shape).  A matrix
- * value that is not finite makes its row's outputs NaN or infinite with fp32
- * activations where fp32 arithmetic would.
+ * with the number of positions (the order of its sum goes by the shape).  Infinities and
+ * NaN in BF16 activations act as in fp32 sums, in fp32 activations too as long as the
+ * matrix row is finite; a matrix value that is not finite makes its row's outputs for
+ * fp32 activations not finite (NaN where an fp32 sum may give an infinity), and in the
+ * fp32 gradient any value that is not finite does so to the outputs that it enters.
  */
 #include <stdint.h>
 
