@@ -171,7 +171,7 @@ int check_workspace(const char* what, const void* ws, uint64_t bytes, uint64_t n
   return K3_SPINE_OK;
 }
 
-// A call of the C surface: nothing that the host code throws leaves it.
+// Nothing that the host code throws leaves the C surface.
 template <typename F>
 int guarded(const char* what, F f) {
   try {
@@ -179,6 +179,15 @@ int guarded(const char* what, F f) {
   } catch (...) {
     return spine_fail(K3_SPINE_E_RUNTIME, "%s: out of host memory", what);
   }
+}
+template <typename F>
+uint64_t guarded_size(const char* what, F f) {
+  uint64_t n = 0;
+  (void)guarded(what, [&] {
+    n = f();
+    return K3_SPINE_OK;
+  });
+  return n;
 }
 
 }  // namespace
@@ -193,42 +202,46 @@ static_assert(sizeof(K3HipGatedGradV1) == 104, "descriptor ABI drift");
 extern "C" {
 
 uint64_t k3_hip_linear_workspace_bytes(const K3HipLinearV1* op) {
-  return check_linear(op, true) == K3_SPINE_OK ? dense_linear_workspace(*op) : 0;
+  if (check_linear(op, true) != K3_SPINE_OK) return 0;
+  return guarded_size("linear", [&] { return dense_linear_workspace(*op); });
 }
 
 int k3_hip_linear(const K3HipLinearV1* op, void* workspace, uint64_t workspace_bytes,
                   void* stream) {
   K3_TRY(check_linear(op, false));
-  K3_TRY(check_workspace("linear", workspace, workspace_bytes, dense_linear_workspace(*op)));
   return guarded("linear", [&] {
+    K3_TRY(check_workspace("linear", workspace, workspace_bytes, dense_linear_workspace(*op)));
     return dense_linear(*op, workspace, static_cast<hipStream_t>(stream));
   });
 }
 
 uint64_t k3_hip_gated_ffn_workspace_bytes(const K3HipGatedV1* op) {
-  return check_gated(op, true) == K3_SPINE_OK ? dense_gated_workspace(*op) : 0;
+  if (check_gated(op, true) != K3_SPINE_OK) return 0;
+  return guarded_size("gated feed-forward", [&] { return dense_gated_workspace(*op); });
 }
 
 int k3_hip_gated_ffn(const K3HipGatedV1* op, void* workspace, uint64_t workspace_bytes,
                      void* stream) {
   K3_TRY(check_gated(op, false));
-  K3_TRY(check_workspace("gated feed-forward", workspace, workspace_bytes,
-                         dense_gated_workspace(*op)));
   return guarded("gated feed-forward", [&] {
+    K3_TRY(check_workspace("gated feed-forward", workspace, workspace_bytes,
+                           dense_gated_workspace(*op)));
     return dense_gated(*op, workspace, static_cast<hipStream_t>(stream));
   });
 }
 
 uint64_t k3_hip_gated_ffn_grad_workspace_bytes(const K3HipGatedGradV1* op) {
-  return check_grad(op, true) == K3_SPINE_OK ? dense_gated_grad_workspace(*op) : 0;
+  if (check_grad(op, true) != K3_SPINE_OK) return 0;
+  return guarded_size("gated feed-forward gradient",
+                      [&] { return dense_gated_grad_workspace(*op); });
 }
 
 int k3_hip_gated_ffn_grad(const K3HipGatedGradV1* op, void* workspace, uint64_t workspace_bytes,
                           void* stream) {
   K3_TRY(check_grad(op, false));
-  K3_TRY(check_workspace("gated feed-forward gradient", workspace, workspace_bytes,
-                         dense_gated_grad_workspace(*op)));
   return guarded("gated feed-forward gradient", [&] {
+    K3_TRY(check_workspace("gated feed-forward gradient", workspace, workspace_bytes,
+                           dense_gated_grad_workspace(*op)));
     return dense_gated_grad(*op, workspace, static_cast<hipStream_t>(stream));
   });
 }

@@ -383,11 +383,11 @@ struct Core {
     const std::true_type yes;
     const std::false_type no;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
-    auto first_half = [&] {  // of the step in the first slots
+    auto first_half = [&](const uint8_t* tw_at, const uint8_t* tx_at) {
       const uint32_t at_w = FW::template place<0>(wn * FN, lane);
       const uint32_t at_x = FX::template place<0>(wm * FM, lane);
 #pragma unroll
-      for (int b = 0; b < FN + FM; ++b) read(h0, b, lds, lds + kSlotX, at_w, at_x);
+      for (int b = 0; b < FN + FM; ++b) read(h0, b, tw_at, tx_at, at_w, at_x);
     };
     auto blocks_there = [] {
       __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): issued a half step ago
@@ -416,7 +416,7 @@ struct Core {
         all_x(lds0 + kSlotX + TX::kBytes);
       }
       if (n > 2) all_w(lds0 + 2 * TW::kBytes);
-      first_half();
+      first_half(lds, lds + kSlotX);
       uint32_t w_at = 0, x_at = kSlotX;  // the step's tiles
       auto next_w = [&] { return w_at == 2 * TW::kBytes ? 0u : w_at + (uint32_t)TW::kBytes; };
       auto next_x = [&] { return 2 * kSlotX + TX::kBytes - x_at; };
@@ -441,16 +441,30 @@ struct Core {
     }
     const int rest = a.k - steps * kStep;
     if (rest > 0 && split == a.splits - 1) {
-      for (segw = segx = 0; segw < a.segments; ++segw, ++segx) {
+      // the segments' rests in turn through two slots, the next one's loads under way
+      auto load_rest = [&](int segment) {
+        segw = segx = segment;
         open_w(steps);
         open_x(steps);
-        __syncthreads();  // the first slots are no longer read
-        tw.load_tail(pw, pu, wave, lane, a.kw - steps * kStep, lds0);
-        tx.load_tail(px, nullptr, wave, lane, a.kx - steps * kStep, lds0 + kSlotX);
-        landed<0>();
-        first_half();
-        half(h0, yes, no, no, lds, lds + kSlotX, 0, 0);
-        half(h1, no, no, no, lds, lds, 0, 0);
+        tw.load_tail(pw, pu, wave, lane, a.kw - steps * kStep, lds0 + (segment & 1) * TW::kBytes);
+        tx.load_tail(px, nullptr, wave, lane, a.kx - steps * kStep,
+                     lds0 + kSlotX + (segment & 1) * TX::kBytes);
+      };
+      __syncthreads();  // the tiles are no longer read
+      load_rest(0);
+      for (int i = 0; i < a.segments; ++i) {
+        if (i + 1 < a.segments) {
+          load_rest(i + 1);
+          landed<TW::kPer + TX::kPer>();
+        } else {
+          landed<0>();
+        }
+        const uint8_t* tw_at = lds + (i & 1) * TW::kBytes;
+        const uint8_t* tx_at = lds + kSlotX + (i & 1) * TX::kBytes;
+        first_half(tw_at, tx_at);
+        half(h0, yes, no, no, tw_at, tx_at, 0, 0);
+        half(h1, no, no, no, tw_at, tx_at, 0, 0);
+        __syncthreads();  // before the load behind the next one
       }
     }
   }

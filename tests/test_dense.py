@@ -168,3 +168,20 @@ def test_oracle_gradient_is_the_difference(act):
             diff[i] = (up - loss(*args)) / (2 * step)
         want = found[{2: 0, 0: 1, 1: 2}[which]]
         assert np.allclose(diff, want, rtol=1e-7, atol=1e-7)
+
+
+def test_c_caller_probe(tmp_path):
+    """The headers as a C11 caller sees them."""
+    import subprocess
+    from pathlib import Path
+
+    from deltafin_amd import _lib
+    root = Path(__file__).resolve().parents[1]
+    exe = tmp_path / "dense_probe"
+    subprocess.run(["gcc", "-std=c11", "-Wall", "-Wextra", "-Werror", f"-I{root / 'include'}",
+                    str(root / "tests" / "c" / "dense_probe.c"), "-o", str(exe),
+                    f"-L{_lib.LIB_PATH.parent}", "-lk3hipmoe",
+                    f"-Wl,-rpath,{_lib.LIB_PATH.parent}"], check=True)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0, r.stderr
+    assert r.stdout.strip() == "ok"
