@@ -377,111 +377,132 @@ __device__ __forceinline__ void terms3(float a, float b, uint32_t (&t)[3]) {
   t[2] = bf16_pair(ra - head_of(t[1], 0), rb - head_of(t[1], 1));
 }
 
-// fp32 rows to three planes [3][rows_out][pitch / 2] (pitch in bytes, zeros past cols and in
-// rows past `rows`); with xs, scaled by the power of two that brings the row's largest
-// finite value into [1, 2), whose inverse goes to xs[row].  A thread takes eight
-// neighbouring values at a time, kHeld such groups of a row in registers between the
-// search for the largest and the split (rows of up to 8192 values are read once).
+// Eight neighbouring fp32 values of a row of `cols` from column 8 g, zeros past its end.
+__device__ __forceinline__ void load_eight(const float* p, int g, int cols, bool aligned,
+                                           float (&v)[8]) {
+  const int c = 8 * g;
+  if (aligned && c + 8 <= cols) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const f32x4 q = *reinterpret_cast<const f32x4*>(p + c + 4 * h);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[4 * h + i] = q[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float value = p[min(c + i, cols - 1)];  // unconditional, as in pack_rows
+      v[i] = c + i < cols ? value : 0.f;
+    }
+  }
+}
+
+// The three terms of eight values to their planes, `plane` bytes apart.
+__device__ __forceinline__ void store_terms(uint8_t* d, uint64_t plane, const float (&v)[8],
+                                            float scale) {
+  u32x4 t[3];
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t p[3];
+    terms3(v[2 * q] * scale, v[2 * q + 1] * scale, p);
+#pragma unroll
+    for (int i = 0; i < 3; ++i) t[i][q] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4*>(d + i * plane) = t[i];
+}
+
+// fp32 rows to three planes [3][rows][pitch / 2] (pitch in bytes, zeros past cols), scaled by
+// the power of two that brings the row's largest finite value into [1, 2), whose inverse
+// goes to xs[row].  A thread takes eight neighbouring values at a time, kHeld such groups of
+// a row in registers between the search for the largest and the split (rows of up to 8192
+// values are read once).
 constexpr int kHeld = 4;
-template <bool kScaled>
 __global__ __launch_bounds__(256) void k_split_rows(const float* __restrict__ x,
                                                     uint8_t* __restrict__ planes,
                                                     float* __restrict__ xs, int rows, int cols,
-                                                    int rows_out, uint32_t pitch, int aligned) {
-  const uint64_t plane = (uint64_t)rows_out * pitch;
+                                                    uint32_t pitch, int aligned) {
+  const uint64_t plane = (uint64_t)rows * pitch;
   __shared__ float red[4];
   const int groups = (int)(pitch / 16);
-  for (int row = blockIdx.x; row < rows_out; row += gridDim.x) {
-    const float* p = x + (uint64_t)min(row, rows - 1) * cols;
-    auto load = [&](int g, float (&v)[8]) {
-      const int c = 8 * g;
-      if (row < rows && aligned && c + 8 <= cols) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const f32x4 q = *reinterpret_cast<const f32x4*>(p + c + 4 * h);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) v[4 * h + i] = q[i];
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float value = p[min(c + i, cols - 1)];  // unconditional, as in k_pack_rows
-          v[i] = row < rows && c + i < cols ? value : 0.f;
-        }
-      }
-    };
+  for (int row = blockIdx.x; row < rows; row += gridDim.x) {
+    const float* p = x + (uint64_t)row * cols;
     float held[kHeld][8];
-    float scale = 1.f;
 #pragma unroll
     for (int k = 0; k < kHeld; ++k) {
       const int g = threadIdx.x + 256 * k;
-      if (g < groups) load(g, held[k]);
+      if (g < groups) load_eight(p, g, cols, aligned, held[k]);
     }
-    if constexpr (kScaled) {
-      float most = 0.f;
-      auto see = [&](const float (&v)[8]) {
+    float most = 0.f;
+    auto see = [&](const float (&v)[8]) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float a = fabsf(v[i]);
-          most = a < INFINITY ? fmaxf(most, a) : most;
-        }
-      };
-#pragma unroll
-      for (int k = 0; k < kHeld; ++k)
-        if ((int)threadIdx.x + 256 * k < groups) see(held[k]);
-      for (int g = threadIdx.x + 256 * kHeld; g < groups; g += 256) {
-        float v[8];
-        load(g, v);
-        see(v);
+      for (int i = 0; i < 8; ++i) {
+        const float a = fabsf(v[i]);
+        most = a < INFINITY ? fmaxf(most, a) : most;
       }
-#pragma unroll
-      for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-      __syncthreads();  // red of the row before
-      if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
-      __syncthreads();
-      most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-      // exponents -126 .. 126, so that the scale and its inverse are normal numbers
-      const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
-      if (most > 0.f) scale = __uint_as_float((uint32_t)(127 - e) << 23);
-      if (threadIdx.x == 0 && row < rows)
-        xs[row] = most > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
-    }
-    uint8_t* d = planes + (uint64_t)row * pitch;
-    auto split = [&](int g, const float (&v)[8]) {
-      u32x4 t[3];
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        uint32_t p[3];
-        terms3(v[2 * q] * scale, v[2 * q + 1] * scale, p);
-#pragma unroll
-        for (int i = 0; i < 3; ++i) t[i][q] = p[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 3; ++i) *reinterpret_cast<u32x4*>(d + i * plane + 16ull * g) = t[i];
     };
 #pragma unroll
+    for (int k = 0; k < kHeld; ++k)
+      if ((int)threadIdx.x + 256 * k < groups) see(held[k]);
+    for (int g = threadIdx.x + 256 * kHeld; g < groups; g += 256) {
+      float v[8];
+      load_eight(p, g, cols, aligned, v);
+      see(v);
+    }
+#pragma unroll
+    for (int d = 32; d > 0; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+    __syncthreads();  // red of the row before
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = most;
+    __syncthreads();
+    most = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    // exponents -126 .. 126, so that the scale and its inverse are normal numbers
+    const int e = min(max((int)(__float_as_uint(most) >> 23) - 127, -126), 126);
+    const float scale = most > 0.f ? __uint_as_float((uint32_t)(127 - e) << 23) : 1.f;
+    if (threadIdx.x == 0)
+      xs[row] = most > 0.f ? __uint_as_float((uint32_t)(127 + e) << 23) : 1.f;
+    uint8_t* d = planes + (uint64_t)row * pitch;
+#pragma unroll
     for (int k = 0; k < kHeld; ++k) {
       const int g = threadIdx.x + 256 * k;
-      if (g < groups) split(g, held[k]);
+      if (g < groups) store_terms(d + 16ull * g, plane, held[k], scale);
     }
     for (int g = threadIdx.x + 256 * kHeld; g < groups; g += 256) {
       float v[8];
-      load(g, v);
-      split(g, v);
+      load_eight(p, g, cols, aligned, v);
+      store_terms(d + 16ull * g, plane, v, scale);
     }
+  }
+}
+
+// fp32 rows to three planes [3][rows_out][pitch / 2] as they are, zeros behind each and in
+// the rows from `rows` on.
+__device__ __forceinline__ void term_rows(const float* __restrict__ x, uint8_t* __restrict__ planes,
+                                          int rows, int cols, int rows_out, uint32_t pitch,
+                                          bool aligned, uint32_t block, uint32_t blocks) {
+  const uint32_t groups = pitch / 16;
+  const uint64_t total = (uint64_t)rows_out * groups, plane = (uint64_t)rows_out * pitch;
+  for (uint64_t t = block * 256ull + threadIdx.x; t < total; t += blocks * 256ull) {
+    const uint64_t row = t / groups;
+    float v[8];
+    load_eight(x + min(row, (uint64_t)rows - 1) * cols, (int)(t - row * groups), cols, aligned, v);
+    if (row >= (uint64_t)rows) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.f;
+    }
+    store_terms(planes + 16 * t, plane, v, 1.f);
   }
 }
 
 // Rows to rows of `pitch` bytes (a multiple of 16), zeros behind each and in the rows from
 // `rows` to rows_out.
 template <typename T>
-__global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u32x4* __restrict__ dst,
-                                                   int rows, int cols, int rows_out,
-                                                   uint32_t pitch) {
+__device__ __forceinline__ void pack_rows(const T* __restrict__ src, u32x4* __restrict__ dst,
+                                          int rows, int cols, int rows_out, uint32_t pitch,
+                                          uint32_t block, uint32_t blocks) {
   constexpr int kPer = 16 / (int)sizeof(T);
   const uint32_t chunks = pitch / 16;
   const uint64_t total = (uint64_t)rows_out * chunks;
-  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
+  for (uint64_t t = block * 256ull + threadIdx.x; t < total; t += blocks * 256ull) {
     const uint64_t row = t / chunks;
     const int c0 = row < (uint64_t)rows ? (int)(t - row * chunks) * kPer : cols;
     const T* p = src + min(row, (uint64_t)rows - 1) * cols;
@@ -496,6 +517,13 @@ __global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u3
     }
     dst[t] = v;
   }
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void k_pack_rows(const T* __restrict__ src, u32x4* __restrict__ dst,
+                                                   int rows, int cols, int rows_out,
+                                                   uint32_t pitch) {
+  pack_rows<T>(src, dst, rows, cols, rows_out, pitch, blockIdx.x, gridDim.x);
 }
 
 // dg = grad f_g(g, u) and du = grad f_u(g, u) of [rows][cols] values as BF16 planes
@@ -520,7 +548,7 @@ __device__ __forceinline__ void load_row_part(const T* p, bool vec, int n, float
   } else {
 #pragma unroll
     for (int i = 0; i < W; ++i) {
-      const float value = widen(p[max(min(i, n - 1), 0)]);  // unconditional, as in k_pack_rows
+      const float value = widen(p[max(min(i, n - 1), 0)]);  // unconditional, as in pack_rows
       v[i] = i < n ? value : 0.f;
     }
   }
@@ -529,15 +557,15 @@ __device__ __forceinline__ void load_row_part(const T* p, bool vec, int n, float
 // W neighbouring columns per thread: eight, or two where eight would leave the card to a few
 // waves that each go through eight sets of exponentials (517 x 1003 fp32 12 us of 105).
 template <typename T, int TERMS, int W>
-__global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, const T* __restrict__ u,
-                                                    const T* __restrict__ grad,
-                                                    uint16_t* __restrict__ planes, int rows,
-                                                    int cols, int rows_out, int half, int act,
-                                                    int vec) {
+__device__ __forceinline__ void gated_grad(const T* __restrict__ g, const T* __restrict__ u,
+                                           const T* __restrict__ grad,
+                                           uint16_t* __restrict__ planes, int rows, int cols,
+                                           int rows_out, int half, int act, int vec,
+                                           uint32_t block, uint32_t blocks) {
   const uint64_t plane = (uint64_t)rows_out * 2 * half;
   const uint32_t groups = (uint32_t)half / W;
   const uint64_t total = (uint64_t)rows_out * groups;
-  for (uint64_t t = blockIdx.x * 256ull + threadIdx.x; t < total; t += gridDim.x * 256ull) {
+  for (uint64_t t = block * 256ull + threadIdx.x; t < total; t += blocks * 256ull) {
     const uint64_t row = t / groups;
     const int c = W * (int)(t - row * groups);
     const int n = row < (uint64_t)rows ? cols - c : 0;
@@ -594,6 +622,52 @@ __global__ __launch_bounds__(256) void k_gated_grad(const T* __restrict__ g, con
   }
 }
 
+// Everything that the gradient's products read and is not in place yet, in one launch of
+// workgroups with a job each: dg and du, copies of the gate, the up matrix and the
+// activations.  One by one the four filled and drained the card for 4 to 8 us each (517
+// rows of 1003 x 2050 in fp32: 23 us together, in one launch 12).
+struct CopyJob {
+  const void* src;
+  uint8_t* dst;
+  int rows, cols, rows_out;
+  uint32_t pitch;
+  uint32_t blocks;  // 0: in place already
+};
+struct GradJob {
+  const void *g, *u, *grad;
+  uint16_t* planes;
+  int rows, cols, rows_out, half, act, vec;
+  uint32_t blocks;
+};
+template <typename T, int TERMS, int W>
+__global__ __launch_bounds__(256) void k_gated_grad(const GradJob d, const CopyJob gate,
+                                                    const CopyJob up, const CopyJob x,
+                                                    int x_aligned) {
+  uint32_t block = blockIdx.x;
+  if (block < d.blocks) {
+    gated_grad<T, TERMS, W>(static_cast<const T*>(d.g), static_cast<const T*>(d.u),
+                            static_cast<const T*>(d.grad), d.planes, d.rows, d.cols, d.rows_out,
+                            d.half, d.act, d.vec, block, d.blocks);
+    return;
+  }
+  block -= d.blocks;
+  if (block < x.blocks) {
+    if constexpr (TERMS == 3)
+      term_rows(static_cast<const float*>(x.src), x.dst, x.rows, x.cols, x.rows_out, x.pitch,
+                x_aligned, block, x.blocks);
+    else
+      pack_rows<uint16_t>(static_cast<const uint16_t*>(x.src), reinterpret_cast<u32x4*>(x.dst),
+                          x.rows, x.cols, x.rows_out, x.pitch, block, x.blocks);
+    return;
+  }
+  block -= x.blocks;
+  const bool second = block >= gate.blocks;
+  const CopyJob& w = second ? up : gate;
+  if (second) block -= gate.blocks;
+  pack_rows<uint16_t>(static_cast<const uint16_t*>(w.src), reinterpret_cast<u32x4*>(w.dst), w.rows,
+                      w.cols, w.rows_out, w.pitch, block, w.blocks);
+}
+
 // ------------------------------------------------------------------ host
 bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
 uint64_t align256(uint64_t v) { return (v + 255) & ~255ull; }
@@ -622,7 +696,7 @@ int launched_or(TimedLaunch& tl, const char* what) {
   return spine_fail(K3_SPINE_E_RUNTIME, "%s: %s", what, hipGetErrorString(err));
 }
 
-int pack_rows(const void* src, void* dst, int elem, int rows, int cols, int rows_out,
+int launch_pack_rows(const void* src, void* dst, int elem, int rows, int cols, int rows_out,
               uint32_t pitch, hipStream_t st) {
   TimedLaunch tl(KC_SPLIT, st);
   const unsigned grid = grid_for((uint64_t)rows_out * (pitch / 16));
@@ -637,17 +711,12 @@ int pack_rows(const void* src, void* dst, int elem, int rows, int cols, int rows
   return launched_or(tl, "dense operand layout");
 }
 
-int split_rows(const void* x, void* planes, float* xs, int rows, int cols, int rows_out,
-               uint32_t pitch, hipStream_t st) {
+int launch_split_rows(const void* x, void* planes, float* xs, int rows, int cols, uint32_t pitch,
+                      hipStream_t st) {
   TimedLaunch tl(KC_SPLIT, st);
-  const dim3 grid((unsigned)std::min(rows_out, 1 << 16));
-  const int aligned = cols % 4 == 0 && aligned16(x);
-  if (xs)
-    launch_timed(tl, k_split_rows<true>, grid, dim3(256), 0, st, static_cast<const float*>(x),
-                 static_cast<uint8_t*>(planes), xs, rows, cols, rows_out, pitch, aligned);
-  else
-    launch_timed(tl, k_split_rows<false>, grid, dim3(256), 0, st, static_cast<const float*>(x),
-                 static_cast<uint8_t*>(planes), xs, rows, cols, rows_out, pitch, aligned);
+  launch_timed(tl, k_split_rows, dim3((unsigned)std::min(rows, 1 << 16)), dim3(256), 0, st,
+               static_cast<const float*>(x), static_cast<uint8_t*>(planes), xs, rows, cols, pitch,
+               (int)(cols % 4 == 0 && aligned16(x)));
   return launched_or(tl, "dense activation terms");
 }
 
@@ -673,7 +742,11 @@ struct Matrix {
   }
   const uint8_t* data() const { return copied ? copy : static_cast<const uint8_t*>(src); }
   int fill(hipStream_t st) const {
-    return copied ? pack_rows(src, copy, elem, rows, cols, rows_out, pitch, st) : K3_SPINE_OK;
+    return copied ? launch_pack_rows(src, copy, elem, rows, cols, rows_out, pitch, st) : K3_SPINE_OK;
+  }
+  CopyJob job() const {
+    const uint32_t blocks = copied ? grid_for((uint64_t)rows_out * (pitch / 16)) : 0;
+    return CopyJob{src, copy, rows, cols, rows_out, pitch, blocks};
   }
 };
 
@@ -701,8 +774,12 @@ struct Activation {
     return planes + (uint64_t)t * rows_out * pitch;
   }
   int fill(hipStream_t st) const {
-    if (f32) return split_rows(src, planes, xs, rows, cols, rows_out, pitch, st);
-    return copied ? pack_rows(src, planes, 2, rows, cols, rows_out, pitch, st) : K3_SPINE_OK;
+    if (f32) return launch_split_rows(src, planes, xs, rows, cols, pitch, st);
+    return copied ? launch_pack_rows(src, planes, 2, rows, cols, rows_out, pitch, st) : K3_SPINE_OK;
+  }
+  CopyJob job() const {
+    const uint32_t blocks = copied ? grid_for((uint64_t)rows_out * (pitch / 16)) : 0;
+    return CopyJob{src, planes, rows, cols, rows_out, pitch, blocks};
   }
 };
 
@@ -1011,29 +1088,25 @@ int dense_gated_grad(const K3HipGatedGradV1& op, void* ws, hipStream_t st) {
   const char* what = "gated feed-forward gradient";
   const bool f32 = op.dtype == K3_DTYPE_F32;
   const int P = (int)op.positions, S = (int)op.rows, H = (int)op.columns;
-  int rc = c.g.fill(st);
-  if (rc == K3_SPINE_OK) rc = c.u.fill(st);
-  if (rc == K3_SPINE_OK) rc = c.x.fill(st);
-  if (rc != K3_SPINE_OK) return rc;
+  int rc;
   {
     TimedLaunch tl(KC_ACTIVATE, st);
-    const int vec = ((uint64_t)S * (f32 ? 4 : 2)) % 16 == 0 && aligned16(op.g) &&
-                    aligned16(op.u) && aligned16(op.grad);
     const uint64_t eights = (uint64_t)c.rows_out * (c.half / 8);
     const bool wide = eights >= 1024ull * std::max(1, device_cu_count());
-    const dim3 grid(grid_for(wide ? eights : 4 * eights));
-    auto go = [&](auto kernel, auto* type) {
-      typedef typename std::remove_pointer<decltype(type)>::type T;
-      launch_timed(tl, kernel, grid, dim3(256), 0, st, static_cast<const T*>(op.g),
-                   static_cast<const T*>(op.u), static_cast<const T*>(op.grad), c.planes, P, S,
-                   c.rows_out, c.half, (int)op.activation, vec);
+    const int vec = ((uint64_t)S * (f32 ? 4 : 2)) % 16 == 0 && aligned16(op.g) &&
+                    aligned16(op.u) && aligned16(op.grad);
+    const GradJob d{op.g, op.u, op.grad, c.planes, P, S, c.rows_out, c.half, (int)op.activation,
+                    vec, grid_for(wide ? eights : 4 * eights)};
+    const CopyJob gate = c.g.job(), up = c.u.job(), x = c.x.job();
+    const int x_aligned = H % 4 == 0 && aligned16(op.x);
+    const dim3 grid(d.blocks + x.blocks + gate.blocks + up.blocks);
+    auto go = [&](auto kernel) {
+      launch_timed(tl, kernel, grid, dim3(256), 0, st, d, gate, up, x, x_aligned);
     };
-    float* f = nullptr;
-    uint16_t* h = nullptr;
     if (f32)
-      wide ? go(k_gated_grad<float, 3, 8>, f) : go(k_gated_grad<float, 3, 2>, f);
+      wide ? go(k_gated_grad<float, 3, 8>) : go(k_gated_grad<float, 3, 2>);
     else
-      wide ? go(k_gated_grad<uint16_t, 1, 8>, h) : go(k_gated_grad<uint16_t, 1, 2>, h);
+      wide ? go(k_gated_grad<uint16_t, 1, 8>) : go(k_gated_grad<uint16_t, 1, 2>);
     if ((rc = launched_or(tl, what)) != K3_SPINE_OK) return rc;
   }
   const uint32_t ldd = 4u * (uint32_t)c.half;  // bytes of a row of dg and du
