@@ -37,7 +37,9 @@ constexpr int kPickThreads = 1024;   // of the workgroup that ends a row
 constexpr double kVanish = 64.0;     // weights under 2^-kVanish round to none
 
 constexpr int kRanges = 4;           // top-k's, top-p's, min-p's and the draw's
-constexpr int kSmall = 64;           // tokens that one wave orders
+constexpr int kSmall = 256;          // tokens that are ranked one against all
+constexpr int kRankers = kPickThreads / kSmall;  // threads per token
+static_assert(kRankers == 4, "their sums meet in two exchanges");
 
 // The ranges of bins in which a row's positions lie; a bin's tokens are gathered for the
 // first of them that holds it.
@@ -546,9 +548,7 @@ struct PickShared {
   uint2 list[kList];
   uint32_t digit_count[256];
   uint64_t digit_mass[256];
-  uint32_t small_key[kSmall];
-  uint32_t small_index[kSmall];
-  uint64_t small_weight[kSmall];
+  ulonglong2 ranked[kSmall];  // key and index, weight
   uint32_t small;
   uint32_t red[2 * kPickThreads / 64];
   uint64_t wave_mass[kPickThreads / 64];
@@ -713,7 +713,7 @@ struct Picker {
     if (part.n > kSmall) narrow(keys, &part);
     while (part.n > kSmall && part.low > 0) digit(keys, by_count, true, target, &part);
     if (part.n <= kSmall) {
-      // few tokens: one wave ranks each against all of them, by key and index
+      // few tokens: four threads rank each against all of them, by key and index
       __syncthreads();
       if (threadIdx.x == 0) sh.small = 0;
       __syncthreads();
@@ -721,27 +721,31 @@ struct Picker {
         if (!in(part, k)) return;
         const uint32_t i = atomicAdd(&sh.small, 1u);
         if (i >= (uint32_t)kSmall) return;  // (the row changed under the call)
-        sh.small_key[i] = k;
-        sh.small_index[i] = t;
-        sh.small_weight[i] = weight(k);
+        sh.ranked[i] = make_ulonglong2((unsigned long long)k << 32 | t, weight(k));
       });
       __syncthreads();
-      if (threadIdx.x < 64) {
-        const int n = min((int)sh.small, kSmall), i = max(min((int)threadIdx.x, n - 1), 0);
-        const uint32_t k = sh.small_key[i], t = sh.small_index[i];
-        const uint64_t w = sh.small_weight[i];
-        uint64_t c = part.before, m = part.mass;
-        for (int j = 0; j < n; ++j) {
-          const uint32_t kj = sh.small_key[j];
-          if (kj < k || (kj == k && sh.small_index[j] < t)) {
-            ++c;
-            m += sh.small_weight[j];
-          }
+      const int n = min((int)sh.small, kSmall), i = threadIdx.x / kRankers;
+      if (i < n) {
+        const ulonglong2 own = sh.ranked[i];
+        uint32_t c = 0;
+        uint64_t m = 0;
+        for (int j = threadIdx.x % kRankers; j < n; j += kRankers) {
+          const ulonglong2 other = sh.ranked[j];
+          const bool ahead = other.x < own.x;
+          c += ahead;
+          m += ahead ? other.y : 0;
         }
-        const uint64_t ahead = by_count ? c : m, here = by_count ? c + 1 : m + w;
-        if ((int)threadIdx.x < n && ahead <= target && here > target) {
-          sh.mass = m + w;
-          sh.token = (int)t;
+#pragma unroll
+        for (int d = 1; d < kRankers; d <<= 1) {
+          c += __shfl_xor(c, d);
+          m += (uint64_t)__shfl_xor((unsigned long long)m, d);
+        }
+        c += part.before;
+        m += part.mass;
+        const uint64_t ahead = by_count ? c : m, here = by_count ? (uint64_t)c + 1 : m + own.y;
+        if (threadIdx.x % kRankers == 0 && ahead <= target && here > target) {
+          sh.mass = m + own.y;
+          sh.token = (int)(uint32_t)own.x;
         }
       }
       __syncthreads();
