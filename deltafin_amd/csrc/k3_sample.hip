@@ -37,7 +37,9 @@ constexpr int kPickThreads = 1024;   // of the workgroup that ends a row
 constexpr double kVanish = 64.0;     // weights under 2^-kVanish round to none
 
 constexpr int kRanges = 4;           // top-k's, top-p's, min-p's and the draw's
-constexpr int kSmall = 256;          // tokens that are ranked one against all
+// Tokens that are ranked one against all: 96 rows of 150001 take 21 us in the last launch;
+// with 64 by one wave 29, 512 27, 1024 26.
+constexpr int kSmall = 256;
 constexpr int kRankers = kPickThreads / kSmall;  // threads per token
 static_assert(kRankers == 4, "their sums meet in two exchanges");
 
