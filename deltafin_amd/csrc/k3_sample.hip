@@ -41,7 +41,8 @@ constexpr int kRanges = 4;           // top-k's, top-p's, min-p's and the draw's
 // with 64 by one wave 29, 512 27, 1024 26.
 constexpr int kSmall = 256;
 constexpr int kRankers = kPickThreads / kSmall;  // threads per token
-static_assert(kRankers == 4, "their sums meet in two exchanges");
+static_assert(kSmall * kRankers == kPickThreads && 64 % kRankers == 0,
+              "a token's threads are in one wave");
 
 // The ranges of bins in which a row's positions lie; a bin's tokens are gathered for the
 // first of them that holds it.
