@@ -299,6 +299,45 @@ def test_gated_backward_integers_are_exact(gpu, positions, rows, cols, dt):
         assert torch.equal(f, want.to(dtype))
 
 
+@pytest.mark.parametrize("dt", ["f32", "bf16"])
+@pytest.mark.parametrize("positions", [37, 128])
+def test_gated_backward_every_alignment_of_views(gpu, positions, dt):
+    """Any of the operands copied, the others in place: sums of small integers, bit for bit
+    (as above)."""
+    import torch
+
+    from deltafin_amd import dense
+    rng = np.random.default_rng(positions)
+    rows, cols = 72, 160
+    dtype = _dt(dt)
+
+    def at(v, dtype, off):
+        flat = torch.full((v.size + off + 8,), float("nan"), dtype=dtype, device="cuda")
+        view = flat[off:off + v.size].view(v.shape)
+        view.copy_(torch.from_numpy(v.astype(np.float32)))
+        return view
+
+    wg, wu = (_ints(rng, (rows, cols), -4, 4) for _ in range(2))
+    x = _ints(rng, (positions, cols), -4, 4)
+    g = 100.0 * rng.integers(0, 2, (positions, rows))
+    u = _ints(rng, (positions, rows), -4, 4)
+    d = _ints(rng, (positions, rows), -1, 1)
+    sig = np.where(g > 0, 1.0, 0.5)
+    dg, du = d * u * sig, d * g * sig
+    wants = [torch.from_numpy(np.asarray(v, np.float64)).to(dtype).cuda()
+             for v in (dg @ wg + du @ wu, dg.T @ x, du.T @ x)]
+    for offs in ((0, 0, 0, 0), (1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (3, 5, 0, 1),
+                 (0, 8, 2, 0), (1, 1, 1, 1)):
+        say(f"backward views {offs} {dt}")
+        og, ou, ox, oa = offs
+        found = dense.gated_ffn_backward(
+            at(wg, torch.bfloat16, og), at(wu, torch.bfloat16, ou), at(x, dtype, ox),
+            at(g, dtype, oa), at(u, dtype, 0), at(d, dtype, oa), "silu")
+        torch.cuda.synchronize()
+        for f, want, name in zip(found, wants, ("d_x", "d_gate", "d_up")):
+            assert torch.equal(f, want), (offs, name)
+
+
 @pytest.mark.parametrize("act", ["silu", "situ"])
 def test_gated_backward_against_differences(gpu, act):
     """Differences of the kernel's own forward pass: a step of 2^-6 along a direction moves

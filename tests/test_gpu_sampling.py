@@ -92,6 +92,34 @@ def test_equal_logits(gpu):
     assert np.array_equal(found, i)
 
 
+@pytest.mark.parametrize("tied", [1, 2, 63, 64, 65, 255, 256, 257, 1000, 4095, 4097])
+def test_groups_of_equal_logits(gpu, tied):
+    """`tied` equal logits among masked ones, at places that no order of the threads gives, a
+    neighbouring value in the same range half as often and a far smaller one.  All weights
+    but the far one's, e^-61, are equal to 2^-22, so u in the middle of a token's share
+    draws that token: over at most 6145 tokens their differences and u's own rounding move a
+    border by under 6145 (2^-22 + 2^-25) = 0.002 of a share."""
+    say(f"{tied} equal logits")
+    rng = np.random.default_rng(tied)
+    vocab = 9001
+    at = rng.permutation(vocab)
+    high, low = np.sort(at[:tied]), np.sort(at[tied:tied + tied // 2])
+    order = np.concatenate([high, low])
+    draws = np.unique(np.concatenate([[0, tied - 1, len(order) - 1],
+                                      rng.integers(0, len(order), 9)]))
+    l = np.full((len(draws), vocab), -np.inf)
+    l[:, high] = 1.0
+    l[:, low] = 1.0 - 2.0 ** -22
+    l[:, at[-1]] = -60.0
+    u = (draws + 0.5) / len(order)
+    found, _ = _run(l, u)
+    assert np.array_equal(found, order[draws])
+    # the same cut behind the equal ones, by count
+    inside = draws[draws < tied]
+    found, _ = _run(l[:len(inside)], (inside + 0.5) / tied, top_k=np.full(len(inside), tied))
+    assert np.array_equal(found, high[inside])
+
+
 def test_masked_and_special(gpu):
     say("masked and special")
     rng = np.random.default_rng(4)
